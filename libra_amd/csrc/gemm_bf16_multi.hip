@@ -13,10 +13,10 @@
 //     b = x (mod 8), i.e. the workgroups of XCD x under the hardware's round-robin placement - so consecutive entries of a queue
 //     go to one XCD at the same time exactly as hardware dispatch would place them, and tile_order's compact per-XCD patches
 //     (hip_common.hpp) keep their L2 sharing.  Every problem starts at a multiple of 8 entries for that reason;
-//   * the first entry of a workgroup is static (t = blockIdx.x); each later one is fetched by ONE returning atomic that is
-//     issued before the tile's prologue loads and read after its epilogue: no fetch latency on the critical path.  (The atomic
-//     is the oldest VMEM operation of the tile, so the prologue's own counted wait covers it: it is issued from inline asm like
-//     the LDS-DMA, DESIGN rule 1, and the compiler's waitcnt pass never sees it.)
+//   * the first entry of a workgroup is static (t = blockIdx.x); each later one is fetched by ONE returning atomic at the
+//     start of the tile before it and read after that tile's epilogue.  (A compiler atomic, which is waited for on the spot, ~1 us
+//     beside a tile's tens - not inline asm: an asm load's result register counts as written at once, so a copy or spill of it
+//     before the data has arrived would hand out a stale entry, and the late write could land in a register reused meanwhile.)
 //   * the queue words live in a 128-byte caller-owned workspace that is all zero between launches: the last workgroup to leave
 //     clears it (no memset node per launch, no library-owned global state).  One workspace per stream.
 //   * a problem may READ the output of one other problem of the same launch (wait_on): its tiles are listed after the producer's,
@@ -85,11 +85,10 @@ __global__ __launch_bounds__(G256_THREADS, 2) void gemm_bf16_multi_kernel(const 
 
 #pragma unroll 1
     for (int t = blockIdx.x; t < nentries;) {
-        // ---- fetch the NEXT entry now (returns the queue's old count), read after the tile
+        // ---- fetch the NEXT entry (returns the queue's old count), read after the tile
         unsigned got = 0;
         if (tid0 == 0) {
-            const unsigned one = 1;
-            asm volatile("global_atomic_add %0, %1, %2, off sc0" : "=v"(got) : "v"(qx), "v"(one) : "memory");
+            got = __hip_atomic_fetch_add(qx, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         // ---- which problem owns entry t (problems are few: a scalar scan)
         int g = 0;
@@ -140,7 +139,6 @@ __global__ __launch_bounds__(G256_THREADS, 2) void gemm_bf16_multi_kernel(const 
             }
         }
         if (tid0 == 0) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // (after a tile: long complete; a pad entry: the fetch's round trip)
             slot[0] = got;
         }
         __syncthreads();                                        // slot visible; the epilogue's LDS slabs are free again
