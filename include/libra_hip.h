@@ -273,6 +273,57 @@ int libra_bridge_attn_decode(const void* q, int64_t ldq, const void* k_same, con
                              int64_t flag_stride, const uint8_t* query_flag, const int* kv_len, const int* kv_start,
                              void* out, int64_t ldo, int64_t B, int64_t H, float scale, float* workspace,
                              size_t workspace_bytes, void* stream);
+/* ---- 8-bit K / V cache (generation) ---------------------------------------------------------------------------------------
+ * The four caches of a layer (K_same, K_cross, V_same, V_cross, see libra_bridge_attn_decode) in one byte a value:
+ *   codes  uint8 [4][B][H][capacity][128]      OCP e4m3 values, head-major (16-byte aligned)
+ *   scales uint8 [4][B][H][capacity / block]   value = code * 2^(scale - 127): one power of two for each `block` tokens and head
+ * block: a power of two, 1..64, that divides capacity.  The scale is the smallest power of two with max|x| <= 448 * scale over the
+ * block's finite values; multiplying by it is exact, so a value is off by at most half a step of e4m3: max(2^-4 |x|, 2^-10 scale).
+ * Infinities saturate, NaN stays NaN.  Half the bytes of the bf16 caches, which bound both batch x context and the step's attention.
+ *
+ * libra_kv8_fill: the S prompt tokens of every sequence (rows [B*S, H*128] bf16, row strides ld_x) into slots [0, S).  Tokens before
+ * kv_start[b] (left padding; NULL: none) are stored as zeros and do not count for the scales; slots >= S are left as they are. */
+int libra_kv8_fill(const void* k_same, int64_t ld_ks, const void* k_cross, int64_t ld_kc, const void* v_same, int64_t ld_vs,
+                   const void* v_cross, int64_t ld_vc, uint8_t* codes, uint8_t* scales, int64_t B, int64_t S, int64_t H,
+                   int64_t capacity, int64_t block, const int32_t* kv_start, void* stream);
+/* libra_kv8_append: one token per sequence (rows [B, H*128]) at slot *slot (device int64: capturable; outside [0, capacity) nothing
+ * is stored).  The first slot of a block sets the block's scale from its token.  A later one keeps the larger of the block's scale and
+ * its own need; where that grows, the codes of the block's earlier slots are re-expressed under the new scale - exact but for values
+ * that leave e4m3's normal range (in all the roundings of a value: at most 2^-9 scale).  Later slots of the block are not touched: a
+ * cache grows from its end, and a slot that is written again makes what lies behind it invalid. */
+int libra_kv8_append(const void* k_same, int64_t ld_ks, const void* k_cross, int64_t ld_kc, const void* v_same, int64_t ld_vs,
+                     const void* v_cross, int64_t ld_vc, uint8_t* codes, uint8_t* scales, int64_t B, int64_t H, int64_t capacity,
+                     int64_t block, const int64_t* slot, void* stream);
+/* libra_kv8_read: tokens [first, first + n) back as bf16 rows, out [4][B*n, H*128] (row stride ldo, buffer stride in elements).  Exact
+ * (an e4m3 number times a power of two has a bf16). */
+int libra_kv8_read(const uint8_t* codes, const uint8_t* scales, void* out, int64_t ldo, int64_t buffer_stride, int64_t B, int64_t H,
+                   int64_t capacity, int64_t block, int64_t first, int64_t n, void* stream);
+/* libra_bridge_attn_decode over the 8-bit cache: one new query token per sequence, key j from the *_cross buffers iff key_flag[b][j] !=
+ * query_flag[b], keys kv_start[b] <= j < kv_len[b] (kv_start NULL: 0; limits outside [0, capacity] are cut to it; no key: zeros).
+ * q, out [B, H*128] bf16, key_flag [B] rows of at least `capacity` flags.  fp32 scores, probabilities and sums.
+ * workspace: >= libra_bridge_attn_decode8_workspace_bytes(B, H), 16-byte aligned: the partial states of the key splits. */
+size_t libra_bridge_attn_decode8_workspace_bytes(int64_t B, int64_t H);
+int libra_bridge_attn_decode8(const void* q, int64_t ldq, const uint8_t* codes, const uint8_t* scales, const uint8_t* key_flag,
+                              int64_t flag_stride, const uint8_t* query_flag, const int32_t* kv_len, const int32_t* kv_start,
+                              void* out, int64_t ldo, int64_t B, int64_t H, int64_t capacity, int64_t block, float scale,
+                              float* workspace, size_t workspace_bytes, void* stream);
+/* ---- log probabilities of given tokens ------------------------------------------------------------------------------------
+ * For every row of logits [rows, V] (bf16, or fp32 with f32 != 0; row stride ldz, any alignment of the element's size):
+ *   logprobs[i][r] = log softmax(z_r)[targets[i][r] - target_sub], i < n_targets (<= 64); 0 for a target < 0 (not scored), -inf for one
+ *                    outside the head's columns (the reference's -inf padded logit)
+ *   stats[0][r] = m_r = max z_r, stats[1][r] = log sum exp(z_r - m_r), stats[2][r] = the entropy of softmax(z_r)
+ *   top_ids[r][k] (+ target_sub), top_logprobs[r][k], k < top (<= 64): the largest logits, equal ones by the smaller column
+ * A row with +inf logits is shared by them (log p = -log n, -inf elsewhere); one of nothing but -inf answers -inf and entropy 0;
+ * one with a NaN answers NaN (the order of its alternatives puts NaN last). */
+int libra_token_logprobs(const void* logits, int64_t ldz, int64_t rows, int64_t V, int f32, const int64_t* targets, int64_t n_targets,
+                         int64_t target_sub, float* logprobs, float* stats, int64_t top, int64_t* top_ids, float* top_logprobs,
+                         void* stream);
+/* dlogits[r][v] = sum_i g_logprobs[i][r] ([v = t_ir] - p_rv) - g_entropy[r] p_rv (log p_rv + H_r), in the logits' type, from the forward's
+ * stats; a target < 0 has no part in it, one outside the columns counts with its -p.  g_logprobs / g_entropy may be NULL.  Rows whose
+ * maximum is infinite get zeros.  dlogits may be the logits themselves (same stride). */
+int libra_token_logprobs_bwd(const void* logits, int64_t ldz, int64_t rows, int64_t V, int f32, const int64_t* targets,
+                             int64_t n_targets, int64_t target_sub, const float* stats, const float* g_logprobs,
+                             const float* g_entropy, void* dlogits, int64_t lddz, void* stream);
 /* Fused routed-bridge causal flash attention, forward (LibraAttention.forward + attn_with_bridge,
  * modeling_libra.py:267-414):  S_ij = q_i.(k_j + [m_i!=m_j] kb_j)/sqrt(d) (+causal, +right padding via
  * kv_len[b] = end of the valid keys, +left padding via kv_start[b] = first valid key; either may be NULL), O_i = sum_j softmax(S)_ij (v_j + [m_i!=m_j] vb_j).  Operands are [B*S, H*128] views with row

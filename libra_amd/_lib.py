@@ -67,6 +67,13 @@ SIGNATURES = {
     "libra_bridge_attn_decode_workspace_bytes": [_I64, _I64],
     "libra_bridge_attn_decode": [_P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F, _P,
                                  C.c_size_t, _P],
+    "libra_kv8_fill": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P],
+    "libra_kv8_append": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P],
+    "libra_kv8_read": [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P],
+    "libra_bridge_attn_decode8_workspace_bytes": [_I64, _I64],
+    "libra_bridge_attn_decode8": [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, C.c_size_t, _P],
+    "libra_token_logprobs": [_P, _I64, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _P, _P, _P],
+    "libra_token_logprobs_bwd": [_P, _I64, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P],
     "libra_bridge_attn_fwd": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _F, _P],
     "libra_bridge_attn_bwd": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64,
                               _P, _P, _P, _P, _I64, _I64, _I64, _I64, _F, _P, _P],
@@ -103,7 +110,7 @@ SIGNATURES = {
     "libra_debug_cu_map": [_P, C.c_int32, C.c_int32, _P],
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 class LibraHipError(RuntimeError):

@@ -6,7 +6,7 @@ autograd runs backward on its own thread).
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import ctypes as C
 import warnings
@@ -995,6 +995,187 @@ def kv_cache_append(rows, caches, slot: torch.Tensor):
                                           caches[0].data_ptr(), caches[1].data_ptr(), caches[2].data_ptr(), caches[3].data_ptr(),
                                           c0.stride(1), c0.stride(0), slot.data_ptr(), B, W, _stream())
     _lib.check(rc, "kv_cache_append")
+
+
+# ---- 8-bit K / V cache (include/libra_hip.h, "8-bit K / V cache") ---------------------------------------------------------------
+KV8_BLOCK = 16             # tokens that share a scale unless a caller chooses otherwise
+
+
+def _here(what: str, *ts) -> None:
+    """Every tensor on the current device: the kernels run on its current stream."""
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            raise ValueError(f"{what}: every tensor must be on the current device (cuda:{dev}), got one on {t.device}")
+
+
+def kv8_alloc(B: int, capacity: int, heads: int, device, block: int = KV8_BLOCK):
+    """(codes uint8 [4, B, heads, capacity', 128], scales uint8 [4, B, heads, capacity' / block]) of one layer, zeroed; capacity' =
+    capacity rounded up to a multiple of `block` (a power of two, 1..64)."""
+    if block < 1 or block > 64 or block & (block - 1):
+        raise ValueError(f"kv8_alloc: block must be a power of two in 1..64, got {block}")
+    cap = round_up(capacity, block)
+    return (torch.zeros((4, B, heads, cap, 128), dtype=torch.uint8, device=device),
+            torch.zeros((4, B, heads, cap // block), dtype=torch.uint8, device=device))
+
+
+def _kv8_geometry(codes: torch.Tensor, scales: torch.Tensor, what: str):
+    """-> (B, H, capacity, block)"""
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 5 or scales.dim() != 4 or codes.shape[0] != 4 \
+            or codes.shape[4] != 128 or codes.shape[:3] != scales.shape[:3] or not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{what}: the cache is contiguous uint8 codes [4, B, H, capacity, 128] and scales [4, B, H, capacity / block], got "
+                         f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+    cap, n = codes.shape[3], scales.shape[3]
+    block = cap // n if n else 0
+    if block * n != cap or block < 1 or block > 64 or block & (block - 1):
+        raise ValueError(f"{what}: capacity {cap} over {n} scales is not a block of 1, 2, 4, ... 64 tokens")
+    return codes.shape[1], codes.shape[2], cap, block
+
+
+def _kv8_rows(rows, n: int, width: int, what: str):
+    if len(rows) != 4:
+        raise ValueError(f"{what}: four row buffers (K_same, K_cross, V_same, V_cross) are expected, got {len(rows)}")
+    for r in rows:
+        _chk2d(r, what + " rows")
+        if r.shape[0] != n or r.shape[1] != width:
+            raise ValueError(f"{what}: rows must be [{n}, {width}], got {tuple(r.shape)}")
+
+
+def kv8_fill(rows, codes: torch.Tensor, scales: torch.Tensor, S: int, *, kv_start: Optional[torch.Tensor] = None) -> None:
+    """Quantise a prompt into slots [0, S): rows = four [B*S, H*128] bf16 tensors (column slices allowed); kv_start int32 [B] (left
+    padding): earlier tokens are stored as zeros and do not count for the scales."""
+    B, H, cap, block = _kv8_geometry(codes, scales, "kv8_fill")
+    _kv8_rows(rows, B * S, H * 128, "kv8_fill")
+    if kv_start is not None and (kv_start.dtype != torch.int32 or kv_start.numel() != B or not kv_start.is_contiguous()):
+        raise ValueError("kv8_fill: kv_start must be contiguous int32 [B]")
+    _here("kv8_fill", codes, scales, kv_start, *rows)
+    rc = _lib.lib().libra_kv8_fill(rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(), rows[1].stride(0), rows[2].data_ptr(),
+                                   rows[2].stride(0), rows[3].data_ptr(), rows[3].stride(0), codes.data_ptr(), scales.data_ptr(), B, S,
+                                   H, cap, block, _ptr(kv_start), _stream())
+    _lib.check(rc, "kv8_fill")
+
+
+def kv8_append(rows, codes: torch.Tensor, scales: torch.Tensor, slot: torch.Tensor) -> None:
+    """Quantise one token per sequence into slot `slot` (cuda int64 [1], read on the device): rows = four [B, H*128] bf16 tensors."""
+    B, H, cap, block = _kv8_geometry(codes, scales, "kv8_append")
+    _kv8_rows(rows, B, H * 128, "kv8_append")
+    if slot.dtype != torch.int64 or slot.numel() != 1:
+        raise ValueError("kv8_append: slot must be a cuda int64 tensor with one element")
+    _here("kv8_append", codes, scales, slot, *rows)
+    rc = _lib.lib().libra_kv8_append(rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(), rows[1].stride(0), rows[2].data_ptr(),
+                                     rows[2].stride(0), rows[3].data_ptr(), rows[3].stride(0), codes.data_ptr(), scales.data_ptr(), B,
+                                     H, cap, block, slot.data_ptr(), _stream())
+    _lib.check(rc, "kv8_append")
+
+
+def kv8_read(codes: torch.Tensor, scales: torch.Tensor, first: int, n: int, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Tokens [first, first + n) as bf16 rows [4, B, n, H*128] (K_same, K_cross, V_same, V_cross) - exactly what the cache stands for."""
+    B, H, cap, block = _kv8_geometry(codes, scales, "kv8_read")
+    if first < 0 or n < 0 or first + n > cap:
+        raise ValueError(f"kv8_read: tokens [{first}, {first + n}) lie outside the cache's {cap}")
+    if out is None:
+        out = torch.empty((4, B, n, H * 128), dtype=BF16, device=codes.device)
+    elif out.dtype != BF16 or tuple(out.shape) != (4, B, n, H * 128) or not out.is_contiguous():
+        raise ValueError(f"kv8_read: out must be contiguous bf16 {(4, B, n, H * 128)}")
+    _here("kv8_read", codes, scales, out)
+    rc = _lib.lib().libra_kv8_read(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), H * 128, B * n * H * 128, B, H, cap, block,
+                                   first, n, _stream())
+    _lib.check(rc, "kv8_read")
+    return out
+
+
+def bridge_attn_decode8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, key_flag: torch.Tensor, query_flag: torch.Tensor,
+                        kv_len: torch.Tensor, scale: float, *, kv_start: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bridge_attn_decode over the 8-bit cache: q [B, H*128] bf16, key_flag [B, >= capacity] u8, query_flag [B] u8, kv_len / kv_start int32
+    [B] -> [B, H*128] bf16."""
+    B, H, cap, block = _kv8_geometry(codes, scales, "bridge_attn_decode8")
+    _chk2d(q, "q")
+    if q.shape[0] != B or q.shape[1] != H * 128:
+        raise ValueError(f"bridge_attn_decode8: q must be [{B}, {H * 128}], got {tuple(q.shape)}")
+    if key_flag.dtype != torch.uint8 or key_flag.dim() != 2 or key_flag.shape[0] != B or key_flag.shape[1] < cap or key_flag.stride(1) != 1 \
+            or query_flag.dtype != torch.uint8 or query_flag.numel() != B or not query_flag.is_contiguous():
+        raise ValueError(f"bridge_attn_decode8: flags are uint8, key_flag [{B}, >= {cap}], query_flag [{B}]")
+    for t, nm in ((kv_len, "kv_len"), (kv_start, "kv_start")):
+        if t is not None and (t.dtype != torch.int32 or t.numel() != B or not t.is_contiguous()):
+            raise ValueError(f"bridge_attn_decode8: {nm} must be contiguous int32 [{B}]")
+    _here("bridge_attn_decode8", q, codes, scales, key_flag, query_flag, kv_len, kv_start)
+    out = torch.empty((B, H * 128), dtype=BF16, device=q.device)
+    nbytes = _lib.lib().libra_bridge_attn_decode8_workspace_bytes(B, H)
+    ws = torch.empty(max(nbytes // 4, 4), dtype=torch.float32, device=q.device)      # partial states of the key splits
+    rc = _lib.lib().libra_bridge_attn_decode8(q.data_ptr(), q.stride(0), codes.data_ptr(), scales.data_ptr(), key_flag.data_ptr(),
+                                              key_flag.stride(0), query_flag.data_ptr(), kv_len.data_ptr(), _ptr(kv_start),
+                                              out.data_ptr(), out.stride(0), B, H, cap, block, float(scale), ws.data_ptr(), nbytes,
+                                              _stream())
+    _lib.check(rc, "bridge_attn_decode8")
+    return out
+
+
+# ---- log probabilities of given tokens (include/libra_hip.h) ------------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' answer: logprobs fp32 [T, rows]; stats fp32 [3, rows] (row maximum, log of the sum of exp(z - maximum), entropy: what
+    the backward takes); top_ids int64 / top_logprobs fp32 [rows, top]."""
+    logprobs: torch.Tensor
+    stats: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+    @property
+    def entropy(self) -> torch.Tensor:
+        return self.stats[2]
+
+    @property
+    def lse(self) -> torch.Tensor:
+        return self.stats[0] + self.stats[1]
+
+
+def _chk_logprobs(logits, targets, what):
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.dtype not in (BF16, torch.float32):
+        raise ValueError(f"{what}: logits must be row-major [rows, V] bf16 or fp32, got {logits.dtype} {tuple(logits.shape)} strides {logits.stride()}")
+    if targets.dtype != torch.int64 or targets.dim() != 2 or targets.shape[1] != logits.shape[0] or not targets.is_contiguous():
+        raise ValueError(f"{what}: targets must be contiguous int64 [T, {logits.shape[0]}], got {targets.dtype} {tuple(targets.shape)}")
+    _here(what, logits, targets)
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, target_sub: int = 0, top: int = 0) -> TokenLogprobs:
+    """Log probability of targets [T, rows] (T tokens per row; < 0: not scored, 0) under softmax(logits [rows, V]), the rows' entropy and
+    their `top` largest logits (<= 64; equal ones by the smaller column).  Token ids are column + target_sub."""
+    _chk_logprobs(logits, targets, "token_logprobs")
+    (rows, V), T = logits.shape, targets.shape[0]
+    if top < 0 or top > min(V, 64):
+        raise ValueError(f"token_logprobs: top must be 0..{min(V, 64)}, got {top}")
+    dev = logits.device
+    lp = torch.empty((T, rows), dtype=torch.float32, device=dev)
+    stats = torch.empty((3, rows), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    tlp = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    rc = _lib.lib().libra_token_logprobs(logits.data_ptr(), logits.stride(0), rows, V, int(logits.dtype == torch.float32),
+                                         targets.data_ptr(), T, target_sub, lp.data_ptr(), stats.data_ptr(), top, ids.data_ptr(),
+                                         tlp.data_ptr(), _stream())
+    _lib.check(rc, "token_logprobs")
+    return TokenLogprobs(lp, stats, ids, tlp)
+
+
+def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, g_logprobs: Optional[torch.Tensor],
+                       g_entropy: Optional[torch.Tensor] = None, *, target_sub: int = 0,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dlogits [rows, V] (the logits' type) from the gradients of logprobs [T, rows] and entropy [rows] (fp32, either may be None)."""
+    _chk_logprobs(logits, targets, "token_logprobs_bwd")
+    (rows, V), T = logits.shape, targets.shape[0]
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (3, rows) or not stats.is_contiguous():
+        raise ValueError(f"token_logprobs_bwd: stats must be the forward's fp32 [3, {rows}]")
+    for t, shape, nm in ((g_logprobs, (T, rows), "g_logprobs"), (g_entropy, (rows,), "g_entropy")):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+            raise ValueError(f"token_logprobs_bwd: {nm} must be contiguous fp32 {shape}")
+    if out is None:
+        out = torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
+    elif out.dtype != logits.dtype or tuple(out.shape) != (rows, V) or out.stride(1) != 1:
+        raise ValueError(f"token_logprobs_bwd: out must be row-major {logits.dtype} {(rows, V)}")
+    _here("token_logprobs_bwd", stats, g_logprobs, g_entropy, out)
+    rc = _lib.lib().libra_token_logprobs_bwd(logits.data_ptr(), logits.stride(0), rows, V, int(logits.dtype == torch.float32),
+                                             targets.data_ptr(), T, target_sub, stats.data_ptr(), _ptr(g_logprobs), _ptr(g_entropy),
+                                             out.data_ptr(), out.stride(0), _stream())
+    _lib.check(rc, "token_logprobs_bwd")
+    return out
 
 
 def bridge_attn_fwd(q, k_same, k_cross, v_same, v_cross, flag, kv_len, B: int, S: int, H: int, scale: float, *,

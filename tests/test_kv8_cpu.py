@@ -1,0 +1,89 @@
+"""The 8-bit K/V cache without a GPU: the 64-bit definition against torch's own e4m3, and what the entry points refuse."""
+import ctypes as C
+
+import pytest
+import torch
+
+import kv8_reference as R
+
+OK, ERR_SHAPE, ERR_ALIGN = 0, -1, -2
+P = C.c_void_p
+FAKE = P(0x10000)            # 16-byte aligned, non-null, never dereferenced
+
+
+def test_reference_grid_is_e4m3():
+    codes = torch.arange(256, dtype=torch.uint8)
+    v, t = R.values(codes), codes.view(torch.float8_e4m3fn).double()
+    assert torch.equal(torch.isnan(v), torch.isnan(t)) and torch.equal(v[~torch.isnan(v)], t[~torch.isnan(t)])
+    x = torch.cat([torch.linspace(-448, 448, 20001), torch.linspace(-0.05, 0.05, 5001), R.GRID.float(), ((R.GRID[1:] + R.GRID[:-1]) / 2).float()])
+    assert torch.equal(R.to_grid(x.double()), x.to(torch.float8_e4m3fn).double())
+
+
+@pytest.mark.parametrize("a,s", [(448.0, 0), (449.0, 1), (1.75, -8), (1.7500001, -7), (1.0, -8), (0.0, -126), (3.0e38, 120), (1e-44, -126)])
+def test_reference_scale(a, s):
+    x = torch.tensor([[a, -a / 2, float("inf"), float("nan")]], dtype=torch.float32).double()
+    assert float(R.shift(x, (1,))) == s
+
+
+@pytest.fixture(scope="module")
+def L():
+    from libra_amd import _lib
+    return _lib.lib()
+
+
+def test_c_entry_points_refuse(L):
+    def fill(**kw):
+        a = dict(dict(ks=FAKE, lk=256, kc=FAKE, lc=256, vs=FAKE, lv=256, vc=FAKE, lw=256, codes=FAKE, scales=FAKE, B=2, S=8, H=2, cap=32,
+                      block=16, start=None, st=None), **kw)
+        return L.libra_kv8_fill(*a.values())
+    assert fill(S=0) == OK and fill(B=0) == OK
+    for bad in (dict(S=33), dict(S=-1), dict(B=-1), dict(H=0), dict(cap=40), dict(block=3), dict(block=0), dict(block=128, cap=128), dict(lk=128),
+                dict(B=70000)):
+        assert fill(**bad) == ERR_SHAPE, bad
+    for bad in (dict(ks=None), dict(vc=P(0x10008)), dict(codes=P(0x10004)), dict(scales=None), dict(lc=260)):
+        assert fill(**bad) == ERR_ALIGN, bad
+
+    def append(**kw):
+        a = dict(dict(ks=FAKE, lk=256, kc=FAKE, lc=256, vs=FAKE, lv=256, vc=FAKE, lw=256, codes=FAKE, scales=FAKE, B=2, H=2, cap=32, block=16,
+                      slot=FAKE, st=None), **kw)
+        return L.libra_kv8_append(*a.values())
+    assert append(B=0) == OK and append(slot=None) == ERR_ALIGN and append(cap=33) == ERR_SHAPE and append(lw=255) == ERR_SHAPE
+
+    def read(**kw):
+        a = dict(dict(codes=FAKE, scales=FAKE, out=FAKE, ldo=256, bs=4096, B=2, H=2, cap=32, block=16, first=0, n=8, st=None), **kw)
+        return L.libra_kv8_read(*a.values())
+    assert read(n=0) == OK and read(first=25) == ERR_SHAPE and read(first=-1) == ERR_SHAPE and read(ldo=128) == ERR_SHAPE
+    assert read(out=None) == ERR_ALIGN and read(ldo=257) == ERR_ALIGN
+
+    ws = L.libra_bridge_attn_decode8_workspace_bytes(2, 2)
+
+    def attn(**kw):
+        a = dict(dict(q=FAKE, ldq=256, codes=FAKE, scales=FAKE, kf=FAKE, fs=32, qf=FAKE, ln=FAKE, start=None, out=FAKE, ldo=256, B=2, H=2,
+                      cap=32, block=16, scale=0.1, ws=FAKE, wsb=ws, st=None), **kw)
+        return L.libra_bridge_attn_decode8(*a.values())
+    assert attn(B=0) == OK
+    for bad in (dict(ldq=128), dict(ldo=128), dict(fs=31), dict(cap=31), dict(block=5), dict(H=-1)):
+        assert attn(**bad) == ERR_SHAPE, bad
+    for bad in (dict(q=None), dict(q=P(0x10008)), dict(kf=None), dict(qf=None), dict(ln=None), dict(out=None), dict(ws=P(0x10004)), dict(wsb=ws - 1),
+                dict(ldq=260)):
+        assert attn(**bad) == ERR_ALIGN, bad
+
+
+def test_host_wrappers_refuse_without_a_gpu():
+    """Shapes, types and devices are judged before anything is launched."""
+    from libra_amd import kernels as K
+    codes, scales = K.kv8_alloc(2, 20, 3, "cpu", 16)
+    assert tuple(codes.shape) == (4, 2, 3, 32, 128) and tuple(scales.shape) == (4, 2, 3, 2)         # capacity rounded up
+    for block in (0, 3, 128, -1):
+        with pytest.raises(ValueError):
+            K.kv8_alloc(1, 8, 1, "cpu", block)
+    assert K._kv8_geometry(codes, scales, "t") == (2, 3, 32, 16)
+    for c, s in ((codes.view(torch.int8), scales), (codes[:, :, :, :31], scales), (codes[..., :64], scales), (codes, scales[:, :1]),
+                 (codes, scales.transpose(0, 1)), (codes[0], scales), (codes, scales[..., :0])):
+        with pytest.raises(ValueError):
+            K._kv8_geometry(c, s, "t")
+    rows = [torch.zeros(2, 384, dtype=torch.bfloat16) for _ in range(4)]
+    with pytest.raises(ValueError):
+        K.kv8_append(rows, codes, scales, torch.zeros(1, dtype=torch.int64))                        # host tensors
+    with pytest.raises(ValueError):
+        K.kv8_append(rows[:3], codes, scales, torch.zeros(1, dtype=torch.int64))
