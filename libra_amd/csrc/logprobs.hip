@@ -18,6 +18,7 @@ template <> struct LpElem<bf16_t> {
     static __device__ __forceinline__ bf16_t put(float v) { return f2bf(v); }
     static __device__ __forceinline__ void unpack(const u32x4 q, float* f) { unpack8(q, f); }
     static __device__ __forceinline__ u32x4 pack(const float* f) { return pack8(f); }
+    static __device__ __forceinline__ u32x4 pack_all(float v) { const unsigned w = pack2bf(v, v); return u32x4{w, w, w, w}; }
 };
 template <> struct LpElem<float> {
     static constexpr int VEC = 4;
@@ -33,6 +34,7 @@ template <> struct LpElem<float> {
         for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(f[i]);
         return q;
     }
+    static __device__ __forceinline__ u32x4 pack_all(float v) { const unsigned w = __float_as_uint(v); return u32x4{w, w, w, w}; }
 };
 // A row is read in 16-byte pieces at 16-byte addresses: piece c holds the columns [c VEC - off, (c + 1) VEC - off), off = how many
 // elements the row begins behind an aligned address (any V and any row stride).  Columns outside the row come as `fill`.
@@ -57,14 +59,24 @@ __device__ __forceinline__ unsigned long long lp_key(float z, int v) {
 }
 __device__ __forceinline__ float lp_diff(float z, float m) { return z == m ? 0.f : z - m; }
 
-constexpr int LP_THREADS = 256;
-template <typename F>
-__device__ __forceinline__ float lp_block(float x, F op, float* red) {
-    for (int o = 32; o > 0; o >>= 1) x = op(x, __shfl_xor(x, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    return op(op(red[0], red[1]), op(red[2], red[3]));
+// the value part of lp_key
+__device__ __forceinline__ unsigned lp_sort(float z) { return (unsigned)(lp_key(z, 0) >> 32); }
+
+template <int N>
+__device__ __forceinline__ float row_ror_fmax(float x) {
+    const unsigned r = (unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x120 + N, 0xf, 0xf, false);
+    return fmaxf(x, __uint_as_float(r));
+}
+// wave-wide maximum / sum: four DPP row rotations and two lane swaps, no trip through LDS
+__device__ __forceinline__ float lp_wave_max(float x) {
+    x = row_ror_fmax<1>(row_ror_fmax<2>(row_ror_fmax<4>(row_ror_fmax<8>(x))));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return half_swap_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float lp_wave_sum(float x) {
+    x = row_ror_add<1>(row_ror_add<2>(row_ror_add<4>(row_ror_add<8>(x))));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
 struct LogprobArgs {
@@ -75,6 +87,255 @@ struct LogprobArgs {
     int top; long long* top_ids; float* top_lp;       // [rows, top]
 };
 
+// A row held in registers: NT threads x NCH pieces of 16 bytes (piece i of thread t = row piece i NT + t), one workgroup a row - the
+// row is read ONCE, its maximum, its sums and its alternatives all come from registers.
+// Alternatives (top <= 64): tau = the largest threshold that at least `top` of the threads' maxima reach (binary search over the bits
+// by one wave, ended early once at most 64 threads do), so at least `top` columns reach it, and only the columns of <= 64 threads can
+// lie above it: those threads lay their pieces into LDS, what reaches tau is listed and ranked by counting.  Where MORE than 64
+// threads' maxima equal tau (rows with masked columns, constant rows), the listed ones are those above tau (of fewer than `top`
+// threads) and the rest are the first columns that equal it, found by a prefix count in column order.
+template <typename T, int NT, int NCH, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
+    typedef LpElem<T> E;
+    constexpr int VEC = E::VEC, NW = NT / 64, NV = NCH * VEC, NEAR = TOP ? 64 : 1, LIST = NEAR * NV;
+    constexpr int LOW = sizeof(T) == 2 ? 16 : 0;                     // lowest bit of the keys that tells two values apart
+    __shared__ float red_m[NW], red_s[NW], red_t[NW];
+    __shared__ unsigned keymax[TOP ? NT : 1];
+    __shared__ u32x4 near_z[TOP ? NEAR * NCH : 1];                   // [NEAR][NCH] pieces of the threads that reach tau, and who they are
+    __shared__ int near_tid[NEAR];
+    __shared__ unsigned long long list[TOP ? LIST : 1];
+    __shared__ unsigned nnear, nlist, tau_s, many_s, wtot[NW];
+    __shared__ int nan_s;
+    const long row = blockIdx.x;
+    const T* z = (const T*)p.z + row * p.ldz;
+    const int off = lp_off(z), tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    u32x4 raw[NCH];
+    const int last = (p.V + off - 1) / VEC;                          // the row's last piece; piece 0 and it may be partial
+    const u32x4 none = E::pack_all(-INFINITY);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int v0 = (i * NT + tid) * VEC - off;
+        raw[i] = none;
+        if (v0 >= 0 && v0 + VEC <= p.V) raw[i] = *(const u32x4*)(z + v0);
+    }
+    if ((tid == 0 && off) || tid == last % NT) {                     // (both may be this thread's: each pass mends one)
+        for (int pass = 0; pass < 2; ++pass) {
+            const int c = pass ? last : 0;
+            if (c % NT != tid) continue;
+            const int v0 = c * VEC - off;
+            if (v0 >= 0 && v0 + VEC <= p.V) continue;
+            float f[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e] = (v0 + e >= 0 && v0 + e < p.V) ? E::get(z[v0 + e]) : -INFINITY;
+            const u32x4 part = E::pack(f);
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) if (i == c / NT) raw[i] = part;
+        }
+    }
+    // the given tokens' logits: requested before the row's own reductions
+    float zt = 0.f;
+    long long tg = -1, tcol = -1;
+    if (tid < p.T) {
+        tg = p.targets[tid * p.rows + row];
+        tcol = tg - p.tsub;
+        if (tg >= 0 && tcol >= 0 && tcol < p.V) zt = E::get(z[tcol]);
+    }
+    if (tid == 0) { nnear = nlist = 0; nan_s = 0; }
+    float mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        float f[VEC];
+        E::unpack(raw[i], f);
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) mine = max3f(mine, f[e], f[e + 1]);
+    }
+    if (TOP) keymax[tid] = lp_sort(mine);
+    float m = lp_wave_max(mine);
+    if (lane == 0) red_m[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, red_m[w]);
+    // (the floats are derived from the packed pieces anew in every phase: kept, they are twice the registers and half the waves)
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) pin(raw[i]);
+    // sum of every exp(z - m), the columns that attain m among them
+    constexpr float L2E = 1.4426950408889634f;
+    float s = 0.f, t = 0.f;
+    if (m < INFINITY && m > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            float f[VEC];
+            E::unpack(raw[i], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = fmaxf(f[e] - m, -1e4f);              // (exp of it is 0 anyway: keeps 0 * -inf out of t; NaN: below)
+                const float ex = __builtin_amdgcn_exp2f(d * L2E);
+                s += ex;
+                t = fmaf(ex, d, t);
+            }
+        }
+    } else {                                                         // a forced row (or one with nothing left): its columns share it
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            float f[VEC];
+            E::unpack(raw[i], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += m > 0.f && f[e] == m ? 1.f : 0.f;
+        }
+    }
+    bool bad = false;                                                // a NaN among the thread's columns: the largest bit pattern of |z| says so
+    {
+        unsigned big = 0;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned w = raw[i][e];
+                if (sizeof(T) == 2) { const unsigned hi = w & 0x7fff0000u, lo = w << 16 & 0x7fff0000u; big = max(big, max(hi, lo)); }
+                else big = max(big, w & 0x7fffffffu);
+            }
+        bad = big > 0x7f800000u;
+    }
+    s = lp_wave_sum(s);
+    t = lp_wave_sum(t);
+    if (lane == 0) { red_s[wave] = s; red_t[wave] = t; }
+    if (bad) nan_s = 1;
+    if (TOP && wave == 0) {                                          // tau, by wave 0
+        unsigned key[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) key[w] = keymax[w * 64 + lane];
+        unsigned tau = 0;
+        int have = NT;
+        for (int bit = 31; bit >= LOW && have > NEAR; --bit) {
+            const unsigned trial = tau | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) n += __popcll(__ballot(key[w] >= trial));
+            if (n >= p.top) { tau = trial; have = n; }
+        }
+        // (the keys of negative bf16 values have ones below LOW, that of NaN, 0, has none: tau becomes the whole key where it is compared
+        //  for equality)
+        if (LOW && have > NEAR && tau && !(tau & 0x80000000u)) tau |= (1u << LOW) - 1;
+        if (lane == 0) { tau_s = tau; many_s = have > NEAR; }
+    }
+    __syncthreads();
+    s = t = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { s += red_s[w]; t += red_t[w]; }
+    const bool nan = nan_s != 0, empty = m == -INFINITY;
+    float r = s - 1.f;
+    if (r < 0.125f && !empty && !nan) {
+        // one column holds nearly everything: the others summed by themselves (a difference of sums near 1 would lose them)
+        float eq = 0.f;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) pin(raw[i]);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            float f[VEC];
+            E::unpack(raw[i], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const bool at = f[e] == m;
+                eq += at ? 1.f : 0.f;
+                s += at ? 0.f : __builtin_amdgcn_exp2f((f[e] - m) * L2E);
+            }
+        }
+        s = lp_wave_sum(s);
+        eq = lp_wave_sum(eq);
+        __syncthreads();                                             // (uniform: every thread has the same r; the old sums are read)
+        if (lane == 0) { red_s[wave] = s; red_m[wave] = eq; }
+        __syncthreads();
+        float rest = 0.f;
+        r = -1.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { r += red_m[w]; rest += red_s[w]; }
+        r += rest;
+    }
+    const float qnan = __uint_as_float(0x7fc00000u);
+    const float lsum = empty ? 0.f : log1pf(r), ent = empty ? 0.f : lsum - t / (1.f + r);
+    auto logp = [&](float zv) { return nan ? qnan : empty ? -INFINITY : lp_diff(zv, m) - lsum; };
+    if (tid == 0) {
+        p.stats[row] = nan ? qnan : m;
+        p.stats[p.rows + row] = nan ? qnan : lsum;
+        p.stats[2 * p.rows + row] = nan ? qnan : ent;
+    }
+    if (tid < p.T) p.logprobs[tid * p.rows + row] = tg < 0 ? 0.f : (tcol >= 0 && tcol < p.V) ? logp(zt) : nan ? qnan : -INFINITY;
+    if constexpr (TOP) {
+        const unsigned tau = tau_s, my = lp_sort(mine);
+        const bool many = many_s != 0;
+        if (many ? my > tau : my >= tau) {                           // <= 64 threads: `have` of them, or fewer than `top`
+            const unsigned at = atomicAdd(&nnear, 1u);
+            if (at < NEAR) {
+                near_tid[at] = tid;
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) near_z[at * NCH + i] = raw[i];
+            }
+        }
+        __syncthreads();
+        const int nn = min((int)nnear, NEAR) * NV;
+        for (int x = tid; x < nn; x += NT) {
+            const int i = x / VEC % NCH, e = x % VEC, at = x / NV;
+            const int v = (i * NT + near_tid[at]) * VEC - off + e;
+            const unsigned long long key = lp_key(E::get(((const T*)near_z)[x]), v);
+            const unsigned u = (unsigned)(key >> 32);
+            if (v >= 0 && v < p.V && (many ? u > tau : u >= tau)) list[atomicAdd(&nlist, 1u)] = key;
+        }
+        __syncthreads();
+        int n = (int)nlist;
+        int need = p.top - n;                                        // > 0 only where many: the first columns that equal tau fill up
+        for (int i = 0; i < NCH && need > 0; ++i) {                  // (uniform; the pieces come from the cache: rare, and one pass nearly always)
+            float f[VEC];
+            lp_load(z, off, p.V, i * NT + tid, 0.f, f);
+            unsigned mask = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int v = (i * NT + tid) * VEC - off + e;
+                mask |= (v >= 0 && v < p.V && lp_sort(f[e]) == tau) ? 1u << e : 0u;
+            }
+            int incl = __popc(mask);
+            for (int o = 1; o < 64; o <<= 1) { const int up = __shfl_up(incl, o, 64); incl += lane >= o ? up : 0; }
+            if (lane == 63) wtot[wave] = (unsigned)incl;
+            __syncthreads();
+            int before = incl - __popc(mask), total = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) { before += w < wave ? (int)wtot[w] : 0; total += (int)wtot[w]; }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (mask >> e & 1) {
+                    if (before < need) list[n + before] = lp_key(f[e], (i * NT + tid) * VEC - off + e);
+                    ++before;
+                }
+            const int got = total < need ? total : need;
+            n += got;
+            need -= got;
+            __syncthreads();
+        }
+        for (int i = tid; i < n; i += NT) {                          // rank = how many listed keys are larger (they are all different)
+            const unsigned long long key = list[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += list[j] > key ? 1 : 0;
+            if (rank < p.top) {
+                const unsigned u = (unsigned)(key >> 32);
+                const float zv = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);              // the key's value (a row with a NaN answers NaN)
+                p.top_ids[row * p.top + rank] = (int)~(unsigned)key + p.tsub;
+                p.top_lp[row * p.top + rank] = logp(zv);
+            }
+        }
+    }
+}
+
+constexpr int LP_THREADS = 256;
+template <typename F>
+__device__ __forceinline__ float lp_block(float x, F op, float* red) {
+    for (int o = 32; o > 0; o >>= 1) x = op(x, __shfl_xor(x, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return op(op(red[0], red[1]), op(red[2], red[3]));
+}
+
+// Rows that no register variant holds (V > ~65 500): the row is read again for each quantity.
 template <typename T>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs p) {
     constexpr int VEC = LpElem<T>::VEC;
@@ -222,6 +483,19 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_bwd_kernel(const LogprobB
 
 using namespace libra;
 
+// the smallest workgroup whose registers hold a row (7 / 3 columns less than the round number: a row may begin behind an aligned address)
+template <typename T, bool TOP>
+static void lp_launch(const LogprobArgs& a, hipStream_t st) {
+    constexpr int W = 8 / LpElem<T>::VEC;                            // pieces are half as wide in fp32
+    const dim3 g((unsigned)a.rows);
+    const int need = a.V + LpElem<T>::VEC - 1;
+    if (need <= 1024) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP>), g, dim3(64), 0, st, a);
+    else if (need <= 8192) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP>), g, dim3(256), 0, st, a);
+    else if (need <= 32768) hipLaunchKernelGGL((logprobs_row_kernel<T, 512, 8 * W, TOP>), g, dim3(512), 0, st, a);
+    else if (need <= 65536) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 8 * W, TOP>), g, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(logprobs_kernel<T>, g, dim3(LP_THREADS), 0, st, a);
+}
+
 static int lp_check(const void* z, int64_t ldz, int64_t rows, int64_t V, int f32, const int64_t* targets, int64_t n_targets) {
     if (rows < 0 || rows > 0x7fffffffL || V <= 0 || V > 0x7ffffff0L || ldz < V || n_targets < 0 || n_targets > 64) return LIBRA_ERR_SHAPE;
     if (!z || ((uintptr_t)z % (f32 ? 4 : 2))) return LIBRA_ERR_ALIGN;
@@ -239,8 +513,10 @@ extern "C" int libra_token_logprobs(const void* logits, int64_t ldz, int64_t row
     if (!stats || (n_targets && !logprobs) || (top && (!top_ids || !top_logprobs))) return LIBRA_ERR_ALIGN;
     LogprobArgs a{logits, (long)ldz, (int)V, (long)rows, (const long long*)targets, (int)n_targets, (long long)target_sub, logprobs, stats,
                   (int)top, (long long*)top_ids, top_logprobs};
-    if (f32) hipLaunchKernelGGL(logprobs_kernel<float>, dim3((unsigned)rows), dim3(LP_THREADS), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(logprobs_kernel<bf16_t>, dim3((unsigned)rows), dim3(LP_THREADS), 0, (hipStream_t)stream, a);
+    const hipStream_t st = (hipStream_t)stream;
+    if (f32) { if (top) lp_launch<float, true>(a, st); else lp_launch<float, false>(a, st); }
+    else if (top) lp_launch<bf16_t, true>(a, st);
+    else lp_launch<bf16_t, false>(a, st);
     return hipGetLastError() == hipSuccess ? LIBRA_OK : LIBRA_ERR_LAUNCH;
 }
 
