@@ -301,8 +301,9 @@ int libra_kv8_read(const uint8_t* codes, const uint8_t* scales, void* out, int64
 /* libra_bridge_attn_decode over the 8-bit cache: one new query token per sequence, key j from the *_cross buffers iff key_flag[b][j] !=
  * query_flag[b], keys kv_start[b] <= j < kv_len[b] (kv_start NULL: 0; limits outside [0, capacity] are cut to it; no key: zeros).
  * q, out [B, H*128] bf16, key_flag [B] rows of at least `capacity` flags.  fp32 scores, probabilities and sums.
- * workspace: >= libra_bridge_attn_decode8_workspace_bytes(B, H), 16-byte aligned: the partial states of the key splits. */
-size_t libra_bridge_attn_decode8_workspace_bytes(int64_t B, int64_t H);
+ * workspace: >= libra_bridge_attn_decode8_workspace_bytes(B, H, capacity), 16-byte aligned: the partial states of the key splits (0 bytes:
+ * none is needed, NULL). */
+size_t libra_bridge_attn_decode8_workspace_bytes(int64_t B, int64_t H, int64_t capacity);
 int libra_bridge_attn_decode8(const void* q, int64_t ldq, const uint8_t* codes, const uint8_t* scales, const uint8_t* key_flag,
                               int64_t flag_stride, const uint8_t* query_flag, const int32_t* kv_len, const int32_t* kv_start,
                               void* out, int64_t ldo, int64_t B, int64_t H, int64_t capacity, int64_t block, float scale,

@@ -1100,11 +1100,11 @@ def bridge_attn_decode8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
             raise ValueError(f"bridge_attn_decode8: {nm} must be contiguous int32 [{B}]")
     _here("bridge_attn_decode8", q, codes, scales, key_flag, query_flag, kv_len, kv_start)
     out = torch.empty((B, H * 128), dtype=BF16, device=q.device)
-    nbytes = _lib.lib().libra_bridge_attn_decode8_workspace_bytes(B, H)
-    ws = torch.empty(max(nbytes // 4, 4), dtype=torch.float32, device=q.device)      # partial states of the key splits
+    nbytes = _lib.lib().libra_bridge_attn_decode8_workspace_bytes(B, H, cap)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None      # partial states of the key splits
     rc = _lib.lib().libra_bridge_attn_decode8(q.data_ptr(), q.stride(0), codes.data_ptr(), scales.data_ptr(), key_flag.data_ptr(),
                                               key_flag.stride(0), query_flag.data_ptr(), kv_len.data_ptr(), _ptr(kv_start),
-                                              out.data_ptr(), out.stride(0), B, H, cap, block, float(scale), ws.data_ptr(), nbytes,
+                                              out.data_ptr(), out.stride(0), B, H, cap, block, float(scale), _ptr(ws), nbytes,
                                               _stream())
     _lib.check(rc, "bridge_attn_decode8")
     return out

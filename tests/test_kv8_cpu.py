@@ -55,14 +55,14 @@ def test_c_entry_points_refuse(L):
     assert read(n=0) == OK and read(first=25) == ERR_SHAPE and read(first=-1) == ERR_SHAPE and read(ldo=128) == ERR_SHAPE
     assert read(out=None) == ERR_ALIGN and read(ldo=257) == ERR_ALIGN
 
-    ws = L.libra_bridge_attn_decode8_workspace_bytes(2, 2)
+    ws = L.libra_bridge_attn_decode8_workspace_bytes(2, 2, 2048)
 
     def attn(**kw):
-        a = dict(dict(q=FAKE, ldq=256, codes=FAKE, scales=FAKE, kf=FAKE, fs=32, qf=FAKE, ln=FAKE, start=None, out=FAKE, ldo=256, B=2, H=2,
-                      cap=32, block=16, scale=0.1, ws=FAKE, wsb=ws, st=None), **kw)
+        a = dict(dict(q=FAKE, ldq=256, codes=FAKE, scales=FAKE, kf=FAKE, fs=2048, qf=FAKE, ln=FAKE, start=None, out=FAKE, ldo=256, B=2, H=2,
+                      cap=2048, block=16, scale=0.1, ws=FAKE, wsb=ws, st=None), **kw)
         return L.libra_bridge_attn_decode8(*a.values())
     assert attn(B=0) == OK
-    for bad in (dict(ldq=128), dict(ldo=128), dict(fs=31), dict(cap=31), dict(block=5), dict(H=-1)):
+    for bad in (dict(ldq=128), dict(ldo=128), dict(fs=2047), dict(cap=2047), dict(block=5), dict(H=-1)):
         assert attn(**bad) == ERR_SHAPE, bad
     for bad in (dict(q=None), dict(q=P(0x10008)), dict(kf=None), dict(qf=None), dict(ln=None), dict(out=None), dict(ws=P(0x10004)), dict(wsb=ws - 1),
                 dict(ldq=260)):
