@@ -25,6 +25,8 @@ struct Decode8Args {
     int B, H, cap, lg; float sl2;                    // scale * log2(e)
     float* part; int nsplit;                         // nsplit > 1: states [B*H][nsplit][D8_PART] instead of `out`
 };
+constexpr int D8_WAVES = 8;
+constexpr int D8_KEYS = 64 * D8_WAVES;               // keys of a workgroup's iteration
 constexpr int D8_MAX_SPLIT = 64;
 constexpr int D8_PART = 132;                         // floats per partial state: 128 outputs, max, sum, 2 pad (rows 16-byte aligned)
 
@@ -47,28 +49,25 @@ __device__ __forceinline__ float groups_sum(float x) {
 }
 // the share of split z of the keys [start, end): whole iterations of a workgroup; splits that get nothing have first >= end
 struct D8Range { int start, end, first, last; };
-template <int WAVES>
 __device__ __forceinline__ D8Range d8_range(const int* lens, const int* starts, int b, int cap, int nsplit, int z) {
-    constexpr int KEYS = 64 * WAVES;                                 // keys of a workgroup's iteration
     D8Range r;
     r.end = min(lens[b], cap);
     r.start = starts ? max(starts[b], 0) : 0;
     const int base = r.start & ~63;
-    const int iters = r.end > r.start ? (r.end - base + KEYS - 1) / KEYS : 0;
+    const int iters = r.end > r.start ? (r.end - base + D8_KEYS - 1) / D8_KEYS : 0;
     const int per = (iters + nsplit - 1) / nsplit;
-    r.first = base + z * per * KEYS;
-    r.last = min(r.first + per * KEYS, r.end);
+    r.first = base + z * per * D8_KEYS;
+    r.last = min(r.first + per * D8_KEYS, r.end);
     return r;
 }
 
-template <int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(const Decode8Args p) {
-    __shared__ float red_m[WAVES], red_l[WAVES];
-    __shared__ __attribute__((aligned(16))) float red_o[WAVES][128];
+__global__ __launch_bounds__(D8_WAVES * 64, 4) void bridge_attn_decode8_kernel(const Decode8Args p) {
+    __shared__ float red_m[D8_WAVES], red_l[D8_WAVES];
+    __shared__ __attribute__((aligned(16))) float red_o[D8_WAVES][128];
     const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 3, sub = lane & 7;                         // 16 channels [16 sub, 16 sub + 16) of keys 8 u + g
-    const D8Range rg = d8_range<WAVES>(p.lens, p.starts, b, p.cap, p.nsplit, z);
+    const D8Range rg = d8_range(p.lens, p.starts, b, p.cap, p.nsplit, z);
     if (rg.first >= rg.last && z > 0) return;                        // (the merge knows; split 0 answers for a sequence without keys)
     const bool vis = p.qflag[b] != 0;
     float qf[16];
@@ -84,7 +83,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(cons
     float m = -INFINITY, l = 0.f, o[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] = 0.f;
-    for (int j0 = rg.first + wave * 64; j0 < rg.last; j0 += WAVES * 64) {
+    for (int j0 = rg.first + wave * 64; j0 < rg.last; j0 += D8_KEYS) {
         // key 8 sub + g of the 64: clamped into the valid ones, so that nothing outside them is ever read
         const int mine = min(max(j0 + 8 * sub + g, rg.start), rg.end - 1);
         const bool cross = (fl[mine] != 0) != vis;
@@ -101,8 +100,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(cons
             kq[u] = *(const u32x4*)at;
             vq[u] = *(const u32x4*)(at + 2 * plane * 128);
         }
-        constexpr bool KEEP = WAVES <= 4;                            // V scales: kept over the softmax, or fetched again where 1024 threads leave
-        float s[8], vs[KEEP ? 8 : 1];                                // 128 registers each (8 less: no spill)
+        float s[8], vs[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             float a = 0.f;
@@ -116,7 +114,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(cons
             }
             const unsigned w = (unsigned)__shfl((int)sc, (lane & 56) | u, 64);
             s[u] = group8_sum(a) * kv8_scale(w >> 8);
-            if (KEEP) vs[u] = kv8_scale(w & 0xff);
+            vs[u] = kv8_scale(w & 0xff);
             if (!whole) { const int j = j0 + 8 * u + g; s[u] = (j >= rg.start && j < rg.end) ? s[u] : -INFINITY; }
         }
         float mn = m;
@@ -132,7 +130,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(cons
         for (int u = 0; u < 8; ++u) {
             const float pr = __builtin_amdgcn_exp2f(s[u] - base);
             l += pr;
-            const float pv = pr * (KEEP ? vs[KEEP ? u : 0] : kv8_scale(__shfl((int)sc, (lane & 56) | u, 64) & 0xff));
+            const float pv = pr * vs[u];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float f[4];
@@ -158,9 +156,9 @@ __global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(cons
     if (threadIdx.x < 128) {
         float M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) M = fmaxf(M, red_m[w]);
+        for (int w = 0; w < D8_WAVES; ++w) M = fmaxf(M, red_m[w]);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
+        for (int w = 0; w < D8_WAVES; ++w) {
             const float f = red_m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(red_m[w] - M);
             L = fmaf(red_l[w], f, L);
             acc = fmaf(red_o[w][threadIdx.x], f, acc);
@@ -176,12 +174,11 @@ __global__ __launch_bounds__(WAVES * 64, 4) void bridge_attn_decode8_kernel(cons
 }
 
 // fold the key splits of one (sequence, head): four waves take every fourth split, two channels a lane (the order is fixed)
-template <int WAVES>
 __global__ __launch_bounds__(256) void bridge_attn_decode8_merge_kernel(const Decode8Args p) {
     __shared__ float acc_s[4][128];
     const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float* pt = p.part + ((long)b * p.H + h) * p.nsplit * D8_PART;
-    const D8Range rg = d8_range<WAVES>(p.lens, p.starts, b, p.cap, p.nsplit, 0);
+    const D8Range rg = d8_range(p.lens, p.starts, b, p.cap, p.nsplit, 0);
     const int per = max(rg.last - rg.first, 1);                      // keys of a full split: split z has some iff first + z per < end
     const int n = rg.end > rg.start ? min(p.nsplit, (rg.end - rg.first + per - 1) / per) : 1;
     float mz = -INFINITY, lz = 0.f;
@@ -210,17 +207,15 @@ __global__ __launch_bounds__(256) void bridge_attn_decode8_merge_kernel(const De
     }
 }
 
-// Waves of a workgroup and key splits of a (sequence, head).  16 waves: one workgroup a CU, its waves merge in LDS, and with 256 or
-// more (sequence, head) pairs there is no second kernel; 4 waves: small workgroups that overlap each other's beginnings and ends.
-struct D8Plan { int waves, nsplit; };
-static D8Plan d8_plan(int64_t B, int64_t H, int64_t capacity) {
-    const int64_t bh = B * H;
-    D8Plan r;
-    r.waves = (bh < 1024 && bh * ((capacity + 1023) / 1024) >= 256) ? 16 : 4;
-    const int64_t keys = 64 * r.waves, target = r.waves == 16 ? 256 : 2048;
-    const int64_t want = (target + bh - 1) / bh, most = (capacity + keys - 1) / keys;
-    r.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), D8_MAX_SPLIT));
-    return r;
+// Key splits of a (sequence, head): 1 - no second kernel - where the pairs alone give every CU a workgroup; below that, as many as that
+// takes, of two iterations at least.  Workgroups of 8 waves, two a CU: of 4, 8 and 16 waves with 1 ... 32 splits the fastest or within
+// 4 % of it at every size tried; at 32 heads, us (waves x splits), HBM floor in brackets:
+//   8 x 1024 [12.9]: 15.4 (8x1) 15.3 (16x1) 19.1 (4x4)    16 x 2048 [51.6]: 50.0 (8x1) 53.3 (16x1) 50.6 (4x1)
+//   32 x 600 [30.2]: 31.8 (8x1) 40.9 (16x1) 31.7 (4x1)    64 x 2048 [206]: 181 (8x1) 189 (16x1) 189 (4x1)
+//   4 x 2048 [12.9]: 18.9 (8x2) 18.7 (16x1) 19.1 (4x4)    1 x 8191 [12.9]: 19.5 (8x8) 19.7 (16x8) 19.6 (4x16) 22.0 (4x32)
+static int d8_splits(int64_t B, int64_t H, int64_t capacity) {
+    const int64_t want = (256 + B * H - 1) / (B * H), most = (capacity + 2 * D8_KEYS - 1) / (2 * D8_KEYS);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), D8_MAX_SPLIT));
 }
 
 }  // namespace libra
@@ -230,7 +225,7 @@ using namespace libra;
 extern "C" int libra_kv8_geometry_(const void* codes, const void* scales, int64_t B, int64_t H, int64_t capacity, int64_t block);
 
 extern "C" size_t libra_bridge_attn_decode8_workspace_bytes(int64_t B, int64_t H, int64_t capacity) {
-    const int n = (B <= 0 || H <= 0 || capacity <= 0) ? 1 : d8_plan(B, H, capacity).nsplit;
+    const int n = (B <= 0 || H <= 0 || capacity <= 0) ? 1 : d8_splits(B, H, capacity);
     return n == 1 ? 0 : (size_t)B * (size_t)H * n * D8_PART * sizeof(float);
 }
 
@@ -250,17 +245,11 @@ extern "C" int libra_bridge_attn_decode8(const void* q, int64_t ldq, const uint8
     a.q = (const bf16_t*)q; a.ldq = ldq; a.codes = codes; a.scales = scales; a.kflag = key_flag; a.fstride = flag_stride;
     a.qflag = query_flag; a.lens = kv_len; a.starts = kv_start; a.out = (bf16_t*)out; a.ldo = ldo;
     a.B = (int)B; a.H = (int)H; a.cap = (int)capacity; a.lg = lg; a.sl2 = scale * 1.4426950408889634f;
-    a.part = workspace;
-    const D8Plan plan = d8_plan(B, H, capacity);
-    a.nsplit = plan.nsplit;
+    a.part = workspace; a.nsplit = d8_splits(B, H, capacity);
     const dim3 grid((unsigned)H, (unsigned)B, (unsigned)a.nsplit), grid2((unsigned)H, (unsigned)B);
     const hipStream_t st = (hipStream_t)stream;
-    if (plan.waves == 16) hipLaunchKernelGGL(bridge_attn_decode8_kernel<16>, grid, dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL(bridge_attn_decode8_kernel<4>, grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(bridge_attn_decode8_kernel, grid, dim3(D8_WAVES * 64), 0, st, a);
     if (hipGetLastError() != hipSuccess) return LIBRA_ERR_LAUNCH;
-    if (a.nsplit > 1) {
-        if (plan.waves == 16) hipLaunchKernelGGL(bridge_attn_decode8_merge_kernel<16>, grid2, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(bridge_attn_decode8_merge_kernel<4>, grid2, dim3(256), 0, st, a);
-    }
+    if (a.nsplit > 1) hipLaunchKernelGGL(bridge_attn_decode8_merge_kernel, grid2, dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? LIBRA_OK : LIBRA_ERR_LAUNCH;
 }
