@@ -94,8 +94,9 @@ struct LogprobArgs {
 // lie above it: those threads lay their pieces into LDS, what reaches tau is listed and ranked by counting.  Where MORE than 64
 // threads' maxima equal tau (rows with masked columns, constant rows), the listed ones are those above tau (of fewer than `top`
 // threads) and the rest are the first columns that equal it, found by a prefix count in column order.
-template <typename T, int NT, int NCH, bool TOP>
-__global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
+template <typename T, int NT, int NCH, bool TOP, int ROWS>
+__global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_row_kernel(const LogprobArgs p) {
+    static_assert(ROWS == 1 || (NT == 64 && !TOP), "several rows a workgroup: a wave each, nothing shared");
     typedef LpElem<T> E;
     constexpr int VEC = E::VEC, NW = NT / 64, NV = NCH * VEC, NEAR = TOP ? 64 : 1, LIST = NEAR * NV;
     constexpr int LOW = sizeof(T) == 2 ? 16 : 0;                     // lowest bit of the keys that tells two values apart
@@ -105,10 +106,10 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
     __shared__ int near_tid[NEAR];
     __shared__ unsigned long long list[TOP ? LIST : 1];
     __shared__ unsigned nnear, nlist, tau_s, many_s, wtot[NW];
-    __shared__ int nan_s;
-    const long row = blockIdx.x;
+    const long row = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x >> 6 : 0);
+    if (ROWS > 1 && row >= p.rows) return;
     const T* z = (const T*)p.z + row * p.ldz;
-    const int off = lp_off(z), tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int off = lp_off(z), tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x, wave = tid >> 6, lane = tid & 63;
     u32x4 raw[NCH];
     const int last = (p.V + off - 1) / VEC;                          // the row's last piece; piece 0 and it may be partial
     const u32x4 none = E::pack_all(-INFINITY);
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
         tcol = tg - p.tsub;
         if (tg >= 0 && tcol >= 0 && tcol < p.V) zt = E::get(z[tcol]);
     }
-    if (tid == 0) { nnear = nlist = 0; nan_s = 0; }
+    if (TOP && tid == 0) nnear = nlist = 0;
     float mine = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -148,58 +149,58 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
         E::unpack(raw[i], f);
 #pragma unroll
         for (int e = 0; e < VEC; e += 2) mine = max3f(mine, f[e], f[e + 1]);
+        __builtin_amdgcn_sched_barrier(0);
     }
     if (TOP) keymax[tid] = lp_sort(mine);
     float m = lp_wave_max(mine);
-    if (lane == 0) red_m[wave] = m;
-    __syncthreads();
+    if (ROWS == 1) {
+        if (lane == 0) red_m[wave] = m;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, red_m[w]);
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, red_m[w]);
+    }
     // (the floats are derived from the packed pieces anew in every phase: kept, they are twice the registers and half the waves)
 #pragma unroll
     for (int i = 0; i < NCH; ++i) pin(raw[i]);
-    // sum of every exp(z - m), the columns that attain m among them
-    constexpr float L2E = 1.4426950408889634f;
+    // s = sum of 2^x, t = sum of 2^x x with x = z log2 e - c, c = m log2 e as rounded: one fused operation a column.  What c's rounding and
+    // log2 e's are off by is a factor common to all columns; it goes out with e_m = 2^x at z = m, by which r and the entropy divide.
+    // (c's rounding stays below 2^-9 for |m| < 16384; beyond that, and for infinite m, x = (z - m) log2 e.)
+    constexpr float L2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+    const float c = m * L2E;
+    const bool close = fabsf(m) < 16384.f;
     float s = 0.f, t = 0.f;
-    if (m < INFINITY && m > -INFINITY) {
+    if (close) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             float f[VEC];
             E::unpack(raw[i], f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float d = fmaxf(f[e] - m, -1e4f);              // (exp of it is 0 anyway: keeps 0 * -inf out of t; NaN: below)
-                const float ex = __builtin_amdgcn_exp2f(d * L2E);
-                s += ex;
-                t = fmaf(ex, d, t);
+                const float x = fmaf(f[e], L2E, -c);
+                const float ex = __builtin_amdgcn_exp2f(x);
+                s += ex;                                             // (NaN iff the row has one)
+                t = fmaf(ex, fmaxf(x, -1e4f), t);                    // (2^x is 0 by then: keeps 0 * -inf out)
             }
+            __builtin_amdgcn_sched_barrier(0);                       // (one piece at a time: 64 exponentials in flight double the registers)
         }
-    } else {                                                         // a forced row (or one with nothing left): its columns share it
+    } else {                                                         // (forced rows, whose infinite columns share them, among these)
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             float f[VEC];
             E::unpack(raw[i], f);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += m > 0.f && f[e] == m ? 1.f : 0.f;
-        }
-    }
-    bool bad = false;                                                // a NaN among the thread's columns: the largest bit pattern of |z| says so
-    {
-        unsigned big = 0;
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned w = raw[i][e];
-                if (sizeof(T) == 2) { const unsigned hi = w & 0x7fff0000u, lo = w << 16 & 0x7fff0000u; big = max(big, max(hi, lo)); }
-                else big = max(big, w & 0x7fffffffu);
+            for (int e = 0; e < VEC; ++e) {
+                const float x = lp_diff(f[e], m) * L2E;
+                const float ex = __builtin_amdgcn_exp2f(x);
+                s += ex;
+                t = fmaf(ex, fmaxf(x, -1e4f), t);
             }
-        bad = big > 0x7f800000u;
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     s = lp_wave_sum(s);
     t = lp_wave_sum(t);
-    if (lane == 0) { red_s[wave] = s; red_t[wave] = t; }
-    if (bad) nan_s = 1;
+    if (ROWS == 1 && lane == 0) { red_s[wave] = s; red_t[wave] = t; }
     if (TOP && wave == 0) {                                          // tau, by wave 0
         unsigned key[NW];
 #pragma unroll
@@ -218,12 +219,15 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
         if (LOW && have > NEAR && tau && !(tau & 0x80000000u)) tau |= (1u << LOW) - 1;
         if (lane == 0) { tau_s = tau; many_s = have > NEAR; }
     }
-    __syncthreads();
-    s = t = 0.f;
+    if (ROWS == 1) {
+        __syncthreads();
+        s = t = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) { s += red_s[w]; t += red_t[w]; }
-    const bool nan = nan_s != 0, empty = m == -INFINITY;
-    float r = s - 1.f;
+        for (int w = 0; w < NW; ++w) { s += red_s[w]; t += red_t[w]; }
+    }
+    const bool nan = s != s, empty = m == -INFINITY;
+    const float xm = close ? fmaf(m, L2E, -c) : 0.f, em = __builtin_amdgcn_exp2f(xm);
+    float r = s - em;
     if (r < 0.125f && !empty && !nan) {
         // one column holds nearly everything: the others summed by themselves (a difference of sums near 1 would lose them)
         float eq = 0.f;
@@ -238,22 +242,26 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(const LogprobArgs p) {
             for (int e = 0; e < VEC; ++e) {
                 const bool at = f[e] == m;
                 eq += at ? 1.f : 0.f;
-                s += at ? 0.f : __builtin_amdgcn_exp2f((f[e] - m) * L2E);
+                s += at ? 0.f : __builtin_amdgcn_exp2f(close ? fmaf(f[e], L2E, -c) : (f[e] - m) * L2E);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         s = lp_wave_sum(s);
         eq = lp_wave_sum(eq);
-        __syncthreads();                                             // (uniform: every thread has the same r; the old sums are read)
-        if (lane == 0) { red_s[wave] = s; red_m[wave] = eq; }
-        __syncthreads();
-        float rest = 0.f;
-        r = -1.f;
+        if (ROWS == 1) {
+            __syncthreads();                                         // (uniform: every thread has the same r; the old sums are read)
+            if (lane == 0) { red_s[wave] = s; red_m[wave] = eq; }
+            __syncthreads();
+            s = eq = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { r += red_m[w]; rest += red_s[w]; }
-        r += rest;
+            for (int w = 0; w < NW; ++w) { eq += red_m[w]; s += red_s[w]; }
+        }
+        r = (eq - 1.f) * em + s;
     }
+    r /= em;                                                         // sum of exp(z - m) beside one column that attains m
     const float qnan = __uint_as_float(0x7fc00000u);
-    const float lsum = empty ? 0.f : log1pf(r), ent = empty ? 0.f : lsum - t / (1.f + r);
+    // H = log1p(r) - sum p (z - m); sum of 2^x (x - xm) = t - xm s, s = em (1 + r)
+    const float lsum = empty ? 0.f : log1pf(r), ent = empty ? 0.f : lsum - LN2 * (t / (em * (1.f + r)) - xm);
     auto logp = [&](float zv) { return nan ? qnan : empty ? -INFINITY : lp_diff(zv, m) - lsum; };
     if (tid == 0) {
         p.stats[row] = nan ? qnan : m;
@@ -434,10 +442,15 @@ struct LogprobBwdArgs {
     void* dz; long lddz;
 };
 
-template <typename T>
-__global__ __launch_bounds__(LP_THREADS) void logprobs_bwd_kernel(const LogprobBwdArgs p) {
-    constexpr int VEC = LpElem<T>::VEC;
-    const long row = blockIdx.x;
+// NT threads a row (ROWS rows a workgroup), every column by itself: x = (z - m - log_sum) log2 e, dz = -2^x (g + g_H (log p + H)).
+// The pieces of a thread that hold a given token (a bit a piece, found first) get that column anew in a rare branch.
+template <typename T, int NT, int ROWS>
+__global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBwdArgs p) {
+    constexpr int VEC = LpElem<T>::VEC, U = 4;
+    constexpr float L2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+    const long row = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / NT : 0);
+    if (ROWS > 1 && row >= p.rows) return;
+    const int tid = ROWS > 1 ? threadIdx.x % NT : threadIdx.x;
     const T* z = (const T*)p.z + row * p.ldz;
     T* dz = (T*)p.dz + row * p.lddz;
     const int off = lp_off(z), nc = (p.V + off + VEC - 1) / VEC;
@@ -446,29 +459,49 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_bwd_kernel(const LogprobB
     const bool flat = m == INFINITY || m == -INFINITY;              // a forced row, or one with nothing left: no gradient
     const float gh = p.g_ent ? p.g_ent[row] : 0.f;
     float g = 0.f;
-    for (int i = 0; i < p.T; ++i) if (p.g_lp && p.targets[i * p.rows + row] >= 0) g += p.g_lp[i * p.rows + row];
-    for (int c = threadIdx.x; c < nc; c += LP_THREADS) {
-        float f[VEC];
-        lp_load(z, off, p.V, c, -INFINITY, f);
+    unsigned long long hits = 0;                                     // bit j: piece tid + j NT holds a given token (63: and all behind it may)
+    if (p.g_lp) {
+        for (int i = 0; i < p.T; ++i) {
+            const long long tg = p.targets[i * p.rows + row], v = tg - p.tsub;
+            if (tg < 0) continue;
+            g += p.g_lp[i * p.rows + row];
+            if (v < 0 || v >= p.V) continue;
+            const int c = (int)((v + off) / VEC), j = c / NT;
+            if (c % NT == tid) hits |= 1ull << (j < 63 ? j : 63);
+        }
+    }
+    const float ls2 = lsum * L2E, a0 = flat ? 0.f : g + gh * ent, a1 = flat ? 0.f : gh * LN2;
+    auto piece = [&](int c, int j, float* f) {
         const int v0 = c * VEC - off;
+        float zk[VEC];
+        const bool hit = (hits >> (j < 63 ? j : 63) & 1) && !flat;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float lp = f[e] - m - lsum, pr = __expf(lp);
-            f[e] = flat ? 0.f : -pr * g - (pr > 0.f ? pr * (lp + ent) * gh : 0.f);
+            zk[e] = f[e];
+            const float x = fmaxf(fmaf(f[e] - m, L2E, -ls2), -1e4f);  // (2^x is 0 by then: keeps 0 * -inf out; a NaN row's a0 is NaN)
+            f[e] = -__builtin_amdgcn_exp2f(x) * fmaf(a1, x, a0);
         }
-        for (int i = 0; i < p.T; ++i) {
-            if (!p.g_lp) break;
-            const long long tg = p.targets[i * p.rows + row], v = tg - p.tsub;
-            if (tg < 0 || v < v0 || v >= v0 + VEC || v < 0 || v >= p.V || flat) continue;
-            // a given token's column anew, with its share as -expm1(log p): 1 - p taken as a difference would lose a sure token's gradient
-            const float lp = LpElem<T>::get(z[v]) - m - lsum, pr = __expf(lp), one = -expm1f(lp);
-            float sum = -(pr > 0.f ? pr * (lp + ent) * gh : 0.f);
-            for (int k = 0; k < p.T; ++k) {
-                const long long tk = p.targets[k * p.rows + row];
-                if (tk >= 0) sum += p.g_lp[k * p.rows + row] * (tk == tg ? one : -pr);
-            }
+        if (hit) {
+            for (int i = 0; i < p.T; ++i) {
+                const long long tg = p.targets[i * p.rows + row], v = tg - p.tsub;
+                if (tg < 0 || v < v0 || v >= v0 + VEC || v < 0 || v >= p.V) continue;
+                float zv = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = (v0 + e == v) ? sum : f[e];
+                for (int e = 0; e < VEC; ++e) zv = v0 + e == v ? zk[e] : zv;
+                // its share as -expm1(log p): 1 - p taken as a difference would lose a sure token's gradient
+                const float lp = zv - m - lsum, pr = __expf(lp), one = -expm1f(lp);
+                float sum = -(pr > 0.f ? pr * (lp + ent) * gh : 0.f);
+                for (int k = 0; k < p.T; ++k) {
+                    const long long tk = p.targets[k * p.rows + row];
+                    if (tk >= 0) sum += p.g_lp[k * p.rows + row] * (tk == tg ? one : -pr);
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f[e] = (v0 + e == v) ? sum : f[e];
+            }
+        }
+        if (flat) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e] = 0.f;
         }
         if (same && v0 >= 0 && v0 + VEC <= p.V) {
             *(u32x4*)(dz + v0) = LpElem<T>::pack(f);
@@ -476,7 +509,30 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_bwd_kernel(const LogprobB
 #pragma unroll
             for (int e = 0; e < VEC; ++e) if (v0 + e >= 0 && v0 + e < p.V) dz[v0 + e] = LpElem<T>::put(f[e]);
         }
+    };
+    int c = tid, j = 0;
+    // U pieces at a time, all of them whole (only piece 0 and the last can be partial): their loads are in flight together
+    for (; c + (U - 1) * NT < nc - 1 && (c > 0 || off == 0); c += U * NT, j += U) {
+        u32x4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = *(const u32x4*)(z + ((c + u * NT) * VEC - off));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[VEC];
+            LpElem<T>::unpack(q[u], f);
+            piece(c + u * NT, j + u, f);
+        }
     }
+    for (; c < nc; c += NT, ++j) {
+        float f[VEC];
+        lp_load(z, off, p.V, c, -INFINITY, f);
+        piece(c, j, f);
+    }
+}
+template <typename T>
+static void lp_launch_bwd(const LogprobBwdArgs& a, hipStream_t st) {
+    if (a.V <= 2048) hipLaunchKernelGGL((logprobs_bwd_kernel<T, 64, 4>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((logprobs_bwd_kernel<T, 256, 1>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
 }
 
 }  // namespace libra
@@ -487,12 +543,13 @@ using namespace libra;
 template <typename T, bool TOP>
 static void lp_launch(const LogprobArgs& a, hipStream_t st) {
     constexpr int W = 8 / LpElem<T>::VEC;                            // pieces are half as wide in fp32
+    constexpr int R = TOP ? 1 : 4;                                   // short rows: four waves, four rows a workgroup
     const dim3 g((unsigned)a.rows);
     const int need = a.V + LpElem<T>::VEC - 1;
-    if (need <= 1024) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP>), g, dim3(64), 0, st, a);
-    else if (need <= 8192) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP>), g, dim3(256), 0, st, a);
-    else if (need <= 32768) hipLaunchKernelGGL((logprobs_row_kernel<T, 512, 8 * W, TOP>), g, dim3(512), 0, st, a);
-    else if (need <= 65536) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 8 * W, TOP>), g, dim3(1024), 0, st, a);
+    if (need <= 1024) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP, R>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(64 * R), 0, st, a);
+    else if (need <= 8192) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP, 1>), g, dim3(256), 0, st, a);
+    else if (need <= 32768) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 4 * W, TOP, 1>), g, dim3(1024), 0, st, a);
+    else if (need <= 65536) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 8 * W, TOP, 1>), g, dim3(1024), 0, st, a);
     else hipLaunchKernelGGL(logprobs_kernel<T>, g, dim3(LP_THREADS), 0, st, a);
 }
 
@@ -530,7 +587,7 @@ extern "C" int libra_token_logprobs_bwd(const void* logits, int64_t ldz, int64_t
     if (!stats || !dlogits || ((uintptr_t)dlogits % (f32 ? 4 : 2)) || (g_logprobs && !targets)) return LIBRA_ERR_ALIGN;
     LogprobBwdArgs a{logits, (long)ldz, (int)V, (long)rows, (const long long*)targets, (int)n_targets, (long long)target_sub, stats,
                      g_logprobs, g_entropy, dlogits, (long)lddz};
-    if (f32) hipLaunchKernelGGL(logprobs_bwd_kernel<float>, dim3((unsigned)rows), dim3(LP_THREADS), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(logprobs_bwd_kernel<bf16_t>, dim3((unsigned)rows), dim3(LP_THREADS), 0, (hipStream_t)stream, a);
+    if (f32) lp_launch_bwd<float>(a, (hipStream_t)stream);
+    else lp_launch_bwd<bf16_t>(a, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? LIBRA_OK : LIBRA_ERR_LAUNCH;
 }
