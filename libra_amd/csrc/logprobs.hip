@@ -36,20 +36,41 @@ template <> struct LpElem<float> {
     }
     static __device__ __forceinline__ u32x4 pack_all(float v) { const unsigned w = __float_as_uint(v); return u32x4{w, w, w, w}; }
 };
-// A row is read in 16-byte pieces at 16-byte addresses: piece c holds the columns [c VEC - off, (c + 1) VEC - off), off = how many
-// elements the row begins behind an aligned address (any V and any row stride).  Columns outside the row come as `fill`.
+// A row is read in 16-byte pieces, piece c = the columns [c VEC, (c + 1) VEC), wherever the row begins (any V, any row stride: the
+// hardware loads 16 bytes at any address of the element's alignment).  The last, partial piece is cut out of the row's last 16 bytes:
+// nothing outside the row is read.  Columns behind the row's end come as -inf.
 template <typename T>
-__device__ __forceinline__ int lp_off(const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); }
+__device__ __forceinline__ u32x4 lp_whole(const T* at) {
+    u32x4 q;
+    __builtin_memcpy(&q, at, 16);
+    return q;
+}
 template <typename T>
-__device__ __forceinline__ void lp_load(const T* row, int off, int V, int c, float fill, float* f) {
+__device__ __forceinline__ u32x4 lp_tail(const T* row, int V, int c) {
     constexpr int VEC = LpElem<T>::VEC;
-    const int v0 = c * VEC - off;
-    if (v0 >= 0 && v0 + VEC <= V) {
-        LpElem<T>::unpack(*(const u32x4*)(row + v0), f);
-    } else {
+    const int v0 = c * VEC;
+    if (V < VEC) {
+        float f[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = (v0 + e >= 0 && v0 + e < V) ? LpElem<T>::get(row[v0 + e]) : fill;
+        for (int e = 0; e < VEC; ++e) f[e] = v0 + e < V ? LpElem<T>::get(row[v0 + e]) : -INFINITY;
+        return LpElem<T>::pack(f);
     }
+    const u32x4 q = lp_whole(row + V - VEC), none = LpElem<T>::pack_all(-INFINITY);
+    const int s = (v0 + VEC - V) * (int)sizeof(T) * 8;               // bits that belong to the piece before: shifted out
+    unsigned long long lo = q[0] | (unsigned long long)q[1] << 32, hi = q[2] | (unsigned long long)q[3] << 32, mlo = ~0ull, mhi = ~0ull;
+    if (s >= 64) { lo = hi; mlo = mhi; hi = mhi = 0; }
+    const int r = s & 63;
+    if (r) {
+        lo = lo >> r | hi << (64 - r); hi >>= r;
+        mlo = mlo >> r | mhi << (64 - r); mhi >>= r;
+    }
+    return u32x4{(unsigned)lo | (none[0] & ~(unsigned)mlo), (unsigned)(lo >> 32) | (none[1] & ~(unsigned)(mlo >> 32)),
+                 (unsigned)hi | (none[2] & ~(unsigned)mhi), (unsigned)(hi >> 32) | (none[3] & ~(unsigned)(mhi >> 32))};
+}
+template <typename T>
+__device__ __forceinline__ void lp_load(const T* row, int V, int c, float* f) {
+    constexpr int VEC = LpElem<T>::VEC;
+    LpElem<T>::unpack((c + 1) * VEC <= V ? lp_whole(row + c * VEC) : c * VEC < V ? lp_tail(row, V, c) : LpElem<T>::pack_all(-INFINITY), f);
 }
 // order of the alternatives: larger value first, then smaller column; NaN behind everything
 __device__ __forceinline__ unsigned long long lp_key(float z, int v) {
@@ -90,10 +111,10 @@ struct LogprobArgs {
 // A row held in registers: NT threads x NCH pieces of 16 bytes (piece i of thread t = row piece i NT + t), one workgroup a row - the
 // row is read ONCE, its maximum, its sums and its alternatives all come from registers.
 // Alternatives (top <= 64): tau = the largest threshold that at least `top` of the threads' maxima reach (binary search over the bits
-// by one wave, ended early once at most 64 threads do), so at least `top` columns reach it, and only the columns of <= 64 threads can
-// lie above it: those threads lay their pieces into LDS, what reaches tau is listed and ranked by counting.  Where MORE than 64
-// threads' maxima equal tau (rows with masked columns, constant rows), the listed ones are those above tau (of fewer than `top`
-// threads) and the rest are the first columns that equal it, found by a prefix count in column order.
+// by one wave, ended early once no more than max(top, 24) do), so at least `top` columns reach it, and only those few threads' columns
+// can: they lay their pieces into LDS, what reaches tau is listed and ranked by counting.  Where the search ends with more threads at
+// tau (rows with masked columns, constant rows: ties), the listed ones are those above tau (of fewer than `top` threads) and the rest
+// are the first columns that equal it, found by a prefix count in column order.
 template <typename T, int NT, int NCH, bool TOP, int ROWS>
 __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_row_kernel(const LogprobArgs p) {
     static_assert(ROWS == 1 || (NT == 64 && !TOP), "several rows a workgroup: a wave each, nothing shared");
@@ -109,29 +130,18 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
     const long row = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x >> 6 : 0);
     if (ROWS > 1 && row >= p.rows) return;
     const T* z = (const T*)p.z + row * p.ldz;
-    const int off = lp_off(z), tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x, wave = tid >> 6, lane = tid & 63;
     u32x4 raw[NCH];
-    const int last = (p.V + off - 1) / VEC;                          // the row's last piece; piece 0 and it may be partial
-    const u32x4 none = E::pack_all(-INFINITY);
+    const int whole = p.V / VEC;                                     // pieces 0 ... whole - 1 are whole, piece `whole` may be partial
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int v0 = (i * NT + tid) * VEC - off;
-        raw[i] = none;
-        if (v0 >= 0 && v0 + VEC <= p.V) raw[i] = *(const u32x4*)(z + v0);
+        raw[i] = E::pack_all(-INFINITY);
+        if (i * NT + tid < whole) raw[i] = lp_whole(z + (i * NT + tid) * VEC);
     }
-    if ((tid == 0 && off) || tid == last % NT) {                     // (both may be this thread's: each pass mends one)
-        for (int pass = 0; pass < 2; ++pass) {
-            const int c = pass ? last : 0;
-            if (c % NT != tid) continue;
-            const int v0 = c * VEC - off;
-            if (v0 >= 0 && v0 + VEC <= p.V) continue;
-            float f[VEC];
+    if (whole * VEC < p.V && tid == whole % NT) {
+        const u32x4 part = lp_tail(z, p.V, whole);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = (v0 + e >= 0 && v0 + e < p.V) ? E::get(z[v0 + e]) : -INFINITY;
-            const u32x4 part = E::pack(f);
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) if (i == c / NT) raw[i] = part;
-        }
+        for (int i = 0; i < NCH; ++i) if (i == whole / NT) raw[i] = part;
     }
     // the given tokens' logits: requested before the row's own reductions
     float zt = 0.f;
@@ -207,7 +217,8 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         for (int w = 0; w < NW; ++w) key[w] = keymax[w * 64 + lane];
         unsigned tau = 0;
         int have = NT;
-        for (int bit = 31; bit >= LOW && have > NEAR; --bit) {
+        const int enough = min(max(p.top, 24), NEAR - 1);            // (fewer to rank, for a few more steps)
+        for (int bit = 31; bit >= LOW && have > enough; --bit) {
             const unsigned trial = tau | (1u << bit);
             int n = 0;
 #pragma unroll
@@ -216,8 +227,8 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         }
         // (the keys of negative bf16 values have ones below LOW, that of NaN, 0, has none: tau becomes the whole key where it is compared
         //  for equality)
-        if (LOW && have > NEAR && tau && !(tau & 0x80000000u)) tau |= (1u << LOW) - 1;
-        if (lane == 0) { tau_s = tau; many_s = have > NEAR; }
+        if (LOW && have > enough && tau && !(tau & 0x80000000u)) tau |= (1u << LOW) - 1;
+        if (lane == 0) { tau_s = tau; many_s = have > enough; }
     }
     if (ROWS == 1) {
         __syncthreads();
@@ -226,12 +237,12 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         for (int w = 0; w < NW; ++w) { s += red_s[w]; t += red_t[w]; }
     }
     const bool nan = s != s, empty = m == -INFINITY;
-    const float xm = close ? fmaf(m, L2E, -c) : 0.f, em = __builtin_amdgcn_exp2f(xm);
+    float xm = close ? fmaf(m, L2E, -c) : 0.f, em = __builtin_amdgcn_exp2f(xm);
     float r = s - em;
     if (r < 0.125f && !empty && !nan) {
-        // one column holds nearly everything: the others summed by themselves (a difference of sums near 1 would lose them)
+        // one column holds nearly everything: the others by themselves, from z - m (differences of sums near 1 would lose them)
         float eq = 0.f;
-        s = 0.f;
+        s = t = 0.f;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) pin(raw[i]);
 #pragma unroll
@@ -241,27 +252,36 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const bool at = f[e] == m;
+                const float x = fmaxf((f[e] - m) * L2E, -1e4f), ex = at ? 0.f : __builtin_amdgcn_exp2f(x);
                 eq += at ? 1.f : 0.f;
-                s += at ? 0.f : __builtin_amdgcn_exp2f(close ? fmaf(f[e], L2E, -c) : (f[e] - m) * L2E);
+                s += ex;
+                t += at ? 0.f : ex * x;
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         s = lp_wave_sum(s);
+        t = lp_wave_sum(t);
         eq = lp_wave_sum(eq);
         if (ROWS == 1) {
             __syncthreads();                                         // (uniform: every thread has the same r; the old sums are read)
-            if (lane == 0) { red_s[wave] = s; red_m[wave] = eq; }
+            if (lane == 0) { red_s[wave] = s; red_t[wave] = t; red_m[wave] = eq; }
             __syncthreads();
-            s = eq = 0.f;
+            s = t = eq = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { eq += red_m[w]; s += red_s[w]; }
+            for (int w = 0; w < NW; ++w) { eq += red_m[w]; s += red_s[w]; t += red_t[w]; }
         }
-        r = (eq - 1.f) * em + s;
+        r = (eq - 1.f) + s;
+        s += eq;
+        em = 1.f;
+        xm = 0.f;
     }
-    r /= em;                                                         // sum of exp(z - m) beside one column that attains m
+    if (!TOP && wave > 0) return;                                    // (what is left is a few numbers a row)
+    const bool sure = r < 0.125f;
+    r *= __builtin_amdgcn_rcpf(em);                                  // sum of exp(z - m) beside one column that attains m
     const float qnan = __uint_as_float(0x7fc00000u);
-    // H = log1p(r) - sum p (z - m); sum of 2^x (x - xm) = t - xm s, s = em (1 + r)
-    const float lsum = empty ? 0.f : log1pf(r), ent = empty ? 0.f : lsum - LN2 * (t / (em * (1.f + r)) - xm);
+    // H = log1p(r) - sum p (z - m), sum p (z - m) = ln 2 (t - xm s) / s
+    const float lsum = empty ? 0.f : sure ? log1pf(r) : __builtin_amdgcn_logf(1.f + r) * LN2;
+    const float ent = empty ? 0.f : lsum - LN2 * (t - xm * s) * __builtin_amdgcn_rcpf(s);
     auto logp = [&](float zv) { return nan ? qnan : empty ? -INFINITY : lp_diff(zv, m) - lsum; };
     if (tid == 0) {
         p.stats[row] = nan ? qnan : m;
@@ -272,7 +292,7 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
     if constexpr (TOP) {
         const unsigned tau = tau_s, my = lp_sort(mine);
         const bool many = many_s != 0;
-        if (many ? my > tau : my >= tau) {                           // <= 64 threads: `have` of them, or fewer than `top`
+        if (many ? my > tau : my >= tau) {                           // <= 64 threads: the `have` of them, or fewer than `top`
             const unsigned at = atomicAdd(&nnear, 1u);
             if (at < NEAR) {
                 near_tid[at] = tid;
@@ -284,22 +304,26 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         const int nn = min((int)nnear, NEAR) * NV;
         for (int x = tid; x < nn; x += NT) {
             const int i = x / VEC % NCH, e = x % VEC, at = x / NV;
-            const int v = (i * NT + near_tid[at]) * VEC - off + e;
+            const int v = (i * NT + near_tid[at]) * VEC + e;
             const unsigned long long key = lp_key(E::get(((const T*)near_z)[x]), v);
             const unsigned u = (unsigned)(key >> 32);
-            if (v >= 0 && v < p.V && (many ? u > tau : u >= tau)) list[atomicAdd(&nlist, 1u)] = key;
+            if (v < p.V && (many ? u > tau : u >= tau)) list[atomicAdd(&nlist, 1u)] = key;
         }
         __syncthreads();
         int n = (int)nlist;
         int need = p.top - n;                                        // > 0 only where many: the first columns that equal tau fill up
-        for (int i = 0; i < NCH && need > 0; ++i) {                  // (uniform; the pieces come from the cache: rare, and one pass nearly always)
+        // (a thread without columns, or with NaNs only, counted as -inf above: where that made tau -inf, NaNs fill what is still missing)
+        for (int k = 0; k < 2 * NCH && need > 0; ++k) {              // (uniform; one pass nearly always, the others' pieces come from the cache)
+            const int i = k < NCH ? k : k - NCH;
+            const unsigned want = k < NCH ? tau : 0u;
             float f[VEC];
-            lp_load(z, off, p.V, i * NT + tid, 0.f, f);
+            if (i == 0) E::unpack(raw[0], f);
+            else lp_load(z, p.V, i * NT + tid, f);
             unsigned mask = 0;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int v = (i * NT + tid) * VEC - off + e;
-                mask |= (v >= 0 && v < p.V && lp_sort(f[e]) == tau) ? 1u << e : 0u;
+                const int v = (i * NT + tid) * VEC + e;
+                mask |= (v < p.V && lp_sort(f[e]) == want) ? 1u << e : 0u;
             }
             int incl = __popc(mask);
             for (int o = 1; o < 64; o <<= 1) { const int up = __shfl_up(incl, o, 64); incl += lane >= o ? up : 0; }
@@ -311,7 +335,7 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 if (mask >> e & 1) {
-                    if (before < need) list[n + before] = lp_key(f[e], (i * NT + tid) * VEC - off + e);
+                    if (before < need) list[n + before] = lp_key(f[e], (i * NT + tid) * VEC + e);
                     ++before;
                 }
             const int got = total < need ? total : need;
@@ -351,15 +375,14 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
     __shared__ unsigned long long redk[4];
     const long row = blockIdx.x;
     const T* z = (const T*)p.z + row * p.ldz;
-    const int off = lp_off(z), nc = (p.V + off + VEC - 1) / VEC;
-    const int tid = threadIdx.x;
+    const int nc = (p.V + VEC - 1) / VEC, tid = threadIdx.x;
     auto maxf = [](float a, float b) { return fmaxf(a, b); };
     auto addf = [](float a, float b) { return a + b; };
     float m = -INFINITY;
     bool nan = false;
     for (int c = tid; c < nc; c += LP_THREADS) {
         float f[VEC];
-        lp_load(z, off, p.V, c, -INFINITY, f);
+        lp_load(z, p.V, c, f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) { nan |= f[e] != f[e]; m = fmaxf(m, f[e]); }
     }
@@ -370,11 +393,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
     float s = 0.f, t = 0.f;
     for (int c = tid; c < nc; c += LP_THREADS) {
         float f[VEC];
-        lp_load(z, off, p.V, c, -INFINITY, f);
+        lp_load(z, p.V, c, f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const int v = c * VEC - off + e;
-            if (v < 0 || v >= p.V) continue;
+            const int v = c * VEC + e;
+            if (v >= p.V) continue;
             const float d = lp_diff(f[e], m);
             if (d == 0.f) { if (v < first) first = v; }
             const float ex = __expf(d);
@@ -385,9 +408,9 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
     int equal = 0;                                     // columns that attain m beyond the first
     for (int c = tid; c < nc; c += LP_THREADS) {
         float f[VEC];
-        lp_load(z, off, p.V, c, -INFINITY, f);
+        lp_load(z, p.V, c, f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { const int v = c * VEC - off + e; equal += (v >= 0 && v < p.V && f[e] == m) ? 1 : 0; }
+        for (int e = 0; e < VEC; ++e) { const int v = c * VEC + e; equal += (v < p.V && f[e] == m) ? 1 : 0; }
     }
     s = lp_block(s, addf, red);
     t = lp_block(t, addf, red);
@@ -412,11 +435,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
         unsigned long long best = 0;
         for (int c = tid; c < nc; c += LP_THREADS) {
             float f[VEC];
-            lp_load(z, off, p.V, c, -INFINITY, f);
+            lp_load(z, p.V, c, f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int v = c * VEC - off + e;
-                if (v < 0 || v >= p.V) continue;
+                const int v = c * VEC + e;
+                if (v >= p.V) continue;
                 const unsigned long long key = lp_key(f[e], v);
                 if (key < last && key > best) best = key;
             }
@@ -453,8 +476,7 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
     const int tid = ROWS > 1 ? threadIdx.x % NT : threadIdx.x;
     const T* z = (const T*)p.z + row * p.ldz;
     T* dz = (T*)p.dz + row * p.lddz;
-    const int off = lp_off(z), nc = (p.V + off + VEC - 1) / VEC;
-    const bool same = lp_off(dz) == off;
+    const int whole = p.V / VEC;                                     // piece `whole` may be partial
     const float m = p.stats[row], lsum = p.stats[p.rows + row], ent = p.stats[2 * p.rows + row];
     const bool flat = m == INFINITY || m == -INFINITY;              // a forced row, or one with nothing left: no gradient
     const float gh = p.g_ent ? p.g_ent[row] : 0.f;
@@ -465,14 +487,14 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
             const long long tg = p.targets[i * p.rows + row], v = tg - p.tsub;
             if (tg < 0) continue;
             g += p.g_lp[i * p.rows + row];
-            if (v < 0 || v >= p.V) continue;
-            const int c = (int)((v + off) / VEC), j = c / NT;
+            if (v >= p.V) continue;
+            const int c = (int)v / VEC, j = c / NT;
             if (c % NT == tid) hits |= 1ull << (j < 63 ? j : 63);
         }
     }
     const float ls2 = lsum * L2E, a0 = flat ? 0.f : g + gh * ent, a1 = flat ? 0.f : gh * LN2;
     auto piece = [&](int c, int j, float* f) {
-        const int v0 = c * VEC - off;
+        const int v0 = c * VEC;
         float zk[VEC];
         const bool hit = (hits >> (j < 63 ? j : 63) & 1) && !flat;
 #pragma unroll
@@ -503,30 +525,32 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
 #pragma unroll
             for (int e = 0; e < VEC; ++e) f[e] = 0.f;
         }
-        if (same && v0 >= 0 && v0 + VEC <= p.V) {
-            *(u32x4*)(dz + v0) = LpElem<T>::pack(f);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) if (v0 + e >= 0 && v0 + e < p.V) dz[v0 + e] = LpElem<T>::put(f[e]);
-        }
     };
     int c = tid, j = 0;
-    // U pieces at a time, all of them whole (only piece 0 and the last can be partial): their loads are in flight together
-    for (; c + (U - 1) * NT < nc - 1 && (c > 0 || off == 0); c += U * NT, j += U) {
+    for (; c + (U - 1) * NT < whole; c += U * NT, j += U) {          // U pieces' loads in flight together
         u32x4 q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = *(const u32x4*)(z + ((c + u * NT) * VEC - off));
+        for (int u = 0; u < U; ++u) q[u] = lp_whole(z + (c + u * NT) * VEC);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[VEC];
             LpElem<T>::unpack(q[u], f);
             piece(c + u * NT, j + u, f);
+            const u32x4 o = LpElem<T>::pack(f);
+            __builtin_memcpy(dz + (c + u * NT) * VEC, &o, 16);
         }
     }
-    for (; c < nc; c += NT, ++j) {
+    for (; c * VEC < p.V; c += NT, ++j) {
         float f[VEC];
-        lp_load(z, off, p.V, c, -INFINITY, f);
+        lp_load(z, p.V, c, f);
         piece(c, j, f);
+        if (c < whole) {
+            const u32x4 o = LpElem<T>::pack(f);
+            __builtin_memcpy(dz + c * VEC, &o, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (c * VEC + e < p.V) dz[c * VEC + e] = LpElem<T>::put(f[e]);
+        }
     }
 }
 template <typename T>
@@ -539,16 +563,16 @@ static void lp_launch_bwd(const LogprobBwdArgs& a, hipStream_t st) {
 
 using namespace libra;
 
-// the smallest workgroup whose registers hold a row (7 / 3 columns less than the round number: a row may begin behind an aligned address)
+// the smallest workgroup whose registers hold a row
 template <typename T, bool TOP>
 static void lp_launch(const LogprobArgs& a, hipStream_t st) {
     constexpr int W = 8 / LpElem<T>::VEC;                            // pieces are half as wide in fp32
     constexpr int R = TOP ? 1 : 4;                                   // short rows: four waves, four rows a workgroup
     const dim3 g((unsigned)a.rows);
-    const int need = a.V + LpElem<T>::VEC - 1;
+    const int need = a.V;
     if (need <= 1024) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP, R>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(64 * R), 0, st, a);
     else if (need <= 8192) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP, 1>), g, dim3(256), 0, st, a);
-    else if (need <= 32768) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 4 * W, TOP, 1>), g, dim3(1024), 0, st, a);
+    else if (need <= 32768) hipLaunchKernelGGL((logprobs_row_kernel<T, 512, 8 * W, TOP, 1>), g, dim3(512), 0, st, a);
     else if (need <= 65536) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 8 * W, TOP, 1>), g, dim3(1024), 0, st, a);
     else hipLaunchKernelGGL(logprobs_kernel<T>, g, dim3(LP_THREADS), 0, st, a);
 }
