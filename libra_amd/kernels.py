@@ -22,7 +22,8 @@ BF16 = torch.bfloat16
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """torch.cuda.current_stream().cuda_stream without building the Stream object: 0.2 us instead of 2.7, once per launch."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -1021,50 +1022,51 @@ def kv8_alloc(B: int, capacity: int, heads: int, device, block: int = KV8_BLOCK)
 
 def _kv8_geometry(codes: torch.Tensor, scales: torch.Tensor, what: str):
     """-> (B, H, capacity, block)"""
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 5 or scales.dim() != 4 or codes.shape[0] != 4 \
-            or codes.shape[4] != 128 or codes.shape[:3] != scales.shape[:3] or not codes.is_contiguous() or not scales.is_contiguous():
+    cs, ss = codes.shape, scales.shape
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or len(cs) != 5 or len(ss) != 4 or cs[0] != 4 or cs[4] != 128 \
+            or cs[:3] != ss[:3] or not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{what}: the cache is contiguous uint8 codes [4, B, H, capacity, 128] and scales [4, B, H, capacity / block], got "
-                         f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
-    cap, n = codes.shape[3], scales.shape[3]
+                         f"{codes.dtype} {tuple(cs)} and {scales.dtype} {tuple(ss)}")
+    cap, n = cs[3], ss[3]
     block = cap // n if n else 0
     if block * n != cap or block < 1 or block > 64 or block & (block - 1):
         raise ValueError(f"{what}: capacity {cap} over {n} scales is not a block of 1, 2, 4, ... 64 tokens")
-    return codes.shape[1], codes.shape[2], cap, block
+    return cs[1], cs[2], cap, block
 
 
 def _kv8_rows(rows, n: int, width: int, what: str):
+    """-> (pointer, row stride) of the four buffers, as the C entry points take them"""
     if len(rows) != 4:
         raise ValueError(f"{what}: four row buffers (K_same, K_cross, V_same, V_cross) are expected, got {len(rows)}")
+    args = []
     for r in rows:
         _chk2d(r, what + " rows")
-        if r.shape[0] != n or r.shape[1] != width:
+        if r.shape != (n, width):
             raise ValueError(f"{what}: rows must be [{n}, {width}], got {tuple(r.shape)}")
+        args += (r.data_ptr(), r.stride(0))
+    return args
 
 
 def kv8_fill(rows, codes: torch.Tensor, scales: torch.Tensor, S: int, *, kv_start: Optional[torch.Tensor] = None) -> None:
     """Quantise a prompt into slots [0, S): rows = four [B*S, H*128] bf16 tensors (column slices allowed); kv_start int32 [B] (left
     padding): earlier tokens are stored as zeros and do not count for the scales."""
     B, H, cap, block = _kv8_geometry(codes, scales, "kv8_fill")
-    _kv8_rows(rows, B * S, H * 128, "kv8_fill")
+    src = _kv8_rows(rows, B * S, H * 128, "kv8_fill")
     if kv_start is not None and (kv_start.dtype != torch.int32 or kv_start.numel() != B or not kv_start.is_contiguous()):
         raise ValueError("kv8_fill: kv_start must be contiguous int32 [B]")
     _here("kv8_fill", codes, scales, kv_start, *rows)
-    rc = _lib.lib().libra_kv8_fill(rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(), rows[1].stride(0), rows[2].data_ptr(),
-                                   rows[2].stride(0), rows[3].data_ptr(), rows[3].stride(0), codes.data_ptr(), scales.data_ptr(), B, S,
-                                   H, cap, block, _ptr(kv_start), _stream())
+    rc = _lib.lib().libra_kv8_fill(*src, codes.data_ptr(), scales.data_ptr(), B, S, H, cap, block, _ptr(kv_start), _stream())
     _lib.check(rc, "kv8_fill")
 
 
 def kv8_append(rows, codes: torch.Tensor, scales: torch.Tensor, slot: torch.Tensor) -> None:
     """Quantise one token per sequence into slot `slot` (cuda int64 [1], read on the device): rows = four [B, H*128] bf16 tensors."""
     B, H, cap, block = _kv8_geometry(codes, scales, "kv8_append")
-    _kv8_rows(rows, B, H * 128, "kv8_append")
+    src = _kv8_rows(rows, B, H * 128, "kv8_append")
     if slot.dtype != torch.int64 or slot.numel() != 1:
         raise ValueError("kv8_append: slot must be a cuda int64 tensor with one element")
     _here("kv8_append", codes, scales, slot, *rows)
-    rc = _lib.lib().libra_kv8_append(rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(), rows[1].stride(0), rows[2].data_ptr(),
-                                     rows[2].stride(0), rows[3].data_ptr(), rows[3].stride(0), codes.data_ptr(), scales.data_ptr(), B,
-                                     H, cap, block, slot.data_ptr(), _stream())
+    rc = _lib.lib().libra_kv8_append(*src, codes.data_ptr(), scales.data_ptr(), B, H, cap, block, slot.data_ptr(), _stream())
     _lib.check(rc, "kv8_append")
 
 
@@ -1074,7 +1076,7 @@ def kv8_read(codes: torch.Tensor, scales: torch.Tensor, first: int, n: int, *, o
     if first < 0 or n < 0 or first + n > cap:
         raise ValueError(f"kv8_read: tokens [{first}, {first + n}) lie outside the cache's {cap}")
     if out is None:
-        out = torch.empty((4, B, n, H * 128), dtype=BF16, device=codes.device)
+        out = codes.new_empty((4, B, n, H * 128), dtype=BF16)
     elif out.dtype != BF16 or tuple(out.shape) != (4, B, n, H * 128) or not out.is_contiguous():
         raise ValueError(f"kv8_read: out must be contiguous bf16 {(4, B, n, H * 128)}")
     _here("kv8_read", codes, scales, out)
@@ -1099,9 +1101,9 @@ def bridge_attn_decode8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
         if t is not None and (t.dtype != torch.int32 or t.numel() != B or not t.is_contiguous()):
             raise ValueError(f"bridge_attn_decode8: {nm} must be contiguous int32 [{B}]")
     _here("bridge_attn_decode8", q, codes, scales, key_flag, query_flag, kv_len, kv_start)
-    out = torch.empty((B, H * 128), dtype=BF16, device=q.device)
+    out = q.new_empty((B, H * 128))
     nbytes = _lib.lib().libra_bridge_attn_decode8_workspace_bytes(B, H, cap)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None      # partial states of the key splits
+    ws = codes.new_empty(nbytes) if nbytes else None      # partial states of the key splits
     rc = _lib.lib().libra_bridge_attn_decode8(q.data_ptr(), q.stride(0), codes.data_ptr(), scales.data_ptr(), key_flag.data_ptr(),
                                               key_flag.stride(0), query_flag.data_ptr(), kv_len.data_ptr(), _ptr(kv_start),
                                               out.data_ptr(), out.stride(0), B, H, cap, block, float(scale), _ptr(ws), nbytes,
@@ -1143,11 +1145,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, target_sub: i
     (rows, V), T = logits.shape, targets.shape[0]
     if top < 0 or top > min(V, 64):
         raise ValueError(f"token_logprobs: top must be 0..{min(V, 64)}, got {top}")
-    dev = logits.device
-    lp = torch.empty((T, rows), dtype=torch.float32, device=dev)
-    stats = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
-    tlp = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    f32 = torch.float32
+    lp, stats, tlp = logits.new_empty((T, rows), dtype=f32), logits.new_empty((3, rows), dtype=f32), logits.new_empty((rows, top), dtype=f32)
+    ids = targets.new_empty((rows, top))
     rc = _lib.lib().libra_token_logprobs(logits.data_ptr(), logits.stride(0), rows, V, int(logits.dtype == torch.float32),
                                          targets.data_ptr(), T, target_sub, lp.data_ptr(), stats.data_ptr(), top, ids.data_ptr(),
                                          tlp.data_ptr(), _stream())
@@ -1167,7 +1167,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, stats: torch
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
             raise ValueError(f"token_logprobs_bwd: {nm} must be contiguous fp32 {shape}")
     if out is None:
-        out = torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty((rows, V))
     elif out.dtype != logits.dtype or tuple(out.shape) != (rows, V) or out.stride(1) != 1:
         raise ValueError(f"token_logprobs_bwd: out must be row-major {logits.dtype} {(rows, V)}")
     _here("token_logprobs_bwd", stats, g_logprobs, g_entropy, out)
