@@ -294,6 +294,12 @@ int libra_kv8_fill(const void* k_same, int64_t ld_ks, const void* k_cross, int64
 int libra_kv8_append(const void* k_same, int64_t ld_ks, const void* k_cross, int64_t ld_kc, const void* v_same, int64_t ld_vs,
                      const void* v_cross, int64_t ld_vc, uint8_t* codes, uint8_t* scales, int64_t B, int64_t H, int64_t capacity,
                      int64_t block, const int64_t* slot, void* stream);
+/* libra_rope_bridge_pos_append with an 8-bit cache: q and K_same rotated in place, the token's four rows quantised into slot *slot as by
+ * libra_kv8_append, in one launch (K_cross and V_cross are not returned). */
+int libra_rope_bridge_pos_append8(void* qkv, int64_t ld, const void* tb, int64_t ldt, const void* bk_l, const void* bk_v,
+                                  const void* bv_l, const void* bv_v, const uint8_t* flag, const void* cos, const void* sin,
+                                  int64_t max_pos, int64_t B, const int* positions, int64_t pos_stride, int64_t H, uint8_t* codes,
+                                  uint8_t* scales, int64_t capacity, int64_t block, const int64_t* slot, void* stream);
 /* libra_kv8_read: tokens [first, first + n) back as bf16 rows, out [4][B*n, H*128] (row stride ldo, buffer stride in elements).  Exact
  * (an e4m3 number times a power of two has a bf16). */
 int libra_kv8_read(const uint8_t* codes, const uint8_t* scales, void* out, int64_t ldo, int64_t buffer_stride, int64_t B, int64_t H,

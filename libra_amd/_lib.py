@@ -69,6 +69,7 @@ SIGNATURES = {
                                  C.c_size_t, _P],
     "libra_kv8_fill": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P],
     "libra_kv8_append": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P],
+    "libra_rope_bridge_pos_append8": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P],
     "libra_kv8_read": [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P],
     "libra_bridge_attn_decode8_workspace_bytes": [_I64, _I64, _I64],
     "libra_bridge_attn_decode8": [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, C.c_size_t, _P],

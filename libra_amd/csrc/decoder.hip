@@ -1,6 +1,6 @@
 // Row kernels of the routed decoder (all HBM-bound): modality-routed RMSNorm, RoPE + rank-8 bridge
 // expansion, SwiGLU, multi-codebook embedding assembly, fused cross-entropy statistics.
-#include "hip_common.hpp"
+#include "kv8.hpp"
 #include "../../include/libra_hip.h"
 
 namespace libra {
@@ -74,6 +74,8 @@ struct RopeArgs {
     // generation step (one token per sequence, token n = sequence n): also store the token's four K / V rows at cache slot *slot
     bf16_t* cache_ks; bf16_t* cache_kc; bf16_t* cache_vs; bf16_t* cache_vc;      // [B, Lmax, H*128] each, or all null
     long c_row, c_batch; const long long* slot;
+    // the same into an 8-bit cache (kv8.hpp): codes [4][N][H][cap][128], scales [4][N][H][cap >> lg]
+    unsigned char* codes; unsigned char* scales; int cap, lg;
 };
 
 __device__ __forceinline__ float rbf(float x) { return bf2f(f2bf(x)); }
@@ -96,6 +98,40 @@ __device__ __forceinline__ u32x2 pack4(const float* f) {
     u32x2 v; v[0] = pack2bf(f[0], f[1]); v[1] = pack2bf(f[2], f[3]); return v;
 }
 
+// One row of one head into an 8-bit cache: the 16 lanes c of a head hold its channels [4c, 4c + 4) and [64 + 4c, 64 + 4c + 4) (x[0], x[1]).
+// The steps of kv8_append: a block's first token sets its scale, a later one that needs more re-expresses the block's earlier codes.
+__device__ __forceinline__ void rope_store8(const RopeArgs& p, int which, long n, int h, int c, int slot, const float (&x)[2][4]) {
+    unsigned mx = 0;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { const unsigned a = kv8_abs_bits(x[hf][e]); mx = a > mx ? a : mx; }
+    int byte = kv8_byte(row16_max(mx));
+    const long head = ((long)which * p.N + n) * p.H + h;
+    unsigned char* sc = p.scales + head * (p.cap >> p.lg) + (slot >> p.lg);
+    unsigned char* dst = p.codes + head * p.cap * 128 + c * 4;
+    const int in_block = slot & ((1 << p.lg) - 1);
+    if (in_block) {
+        const int old = min((int)sc[0], 254);
+        if (byte > old) {
+            const float down = kv8_scale(max(127 + old - byte, 0));
+            for (long t = slot - in_block; t < slot; ++t) {
+                unsigned* w = (unsigned*)(dst + t * 128);
+                w[0] = kv8_rescale4(w[0], down);
+                w[16] = kv8_rescale4(w[16], down);
+            }
+        } else {
+            byte = old;
+        }
+    }
+    const float inv = kv8_inverse(byte);
+    unsigned* w = (unsigned*)(dst + (long)slot * 128);
+    w[0] = kv8_encode4(x[0][0] * inv, x[0][1] * inv, x[0][2] * inv, x[0][3] * inv);
+    w[16] = kv8_encode4(x[1][0] * inv, x[1][1] * inv, x[1][2] * inv, x[1][3] * inv);
+    if (c == 0) sc[0] = (unsigned char)byte;
+}
+
+template <bool Q8>
 __global__ __launch_bounds__(256) void rope_bridge_kernel(const RopeArgs p) {
     const int LT = p.H * 16;                                  // threads per token
     const int tpb = LT >= 256 ? 1 : 256 / LT;                 // token slots per block
@@ -162,6 +198,24 @@ __global__ __launch_bounds__(256) void rope_bridge_kernel(const RopeArgs p) {
             kc[1][e] = rbf(rbf(kx1 * cs[1][e]) + rbf(kx0 * sn[1][e]));
             vc[0][e] = v[0][e] + vb[0][e];
             vc[1][e] = v[1][e] + vb[1][e];
+        }
+        if constexpr (Q8) {                                   // generation step, 8-bit cache: q and K_same in place, the rows into the cache
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const long col = (long)h * 128 + hf * 64 + c * 4;
+                *(u32x2*)(p.qkv + n * p.ld + col) = pack4(qo[hf]);
+                *(u32x2*)(p.qkv + n * p.ld + HD + col) = pack4(ko[hf]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) vc[hf][e] = rbf(vc[hf][e]);
+            }
+            const long long slot = p.slot[0];
+            if (slot >= 0 && slot < p.cap) {
+                rope_store8(p, 0, n, h, c, (int)slot, ko);
+                rope_store8(p, 1, n, h, c, (int)slot, kc);
+                rope_store8(p, 2, n, h, c, (int)slot, v);
+                rope_store8(p, 3, n, h, c, (int)slot, vc);
+            }
+            continue;
         }
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
@@ -328,7 +382,8 @@ static int rope_bridge_run(void* qkv, int64_t ld, const void* tb, int64_t ldt, c
                            const void* bv_l, const void* bv_v, const uint8_t* flag, const void* cos, const void* sin,
                            int64_t max_pos, void* k_cross, void* v_cross, int64_t ldc, int64_t N, int64_t S,
                            int64_t H, const int* positions, int64_t pos_stride, void* stream, void* const* cache = nullptr,
-                           int64_t c_row = 0, int64_t c_batch = 0, const int64_t* slot = nullptr) {
+                           int64_t c_row = 0, int64_t c_batch = 0, const int64_t* slot = nullptr, uint8_t* codes = nullptr,
+                           uint8_t* scales = nullptr, int64_t capacity = 0, int lg = 0) {
     if (N <= 0) return LIBRA_OK;
     if (cache) {
         if (!slot || c_row < H * 128 || c_batch < c_row || (c_row % 8) || (c_batch % 8)) return LIBRA_ERR_SHAPE;
@@ -337,7 +392,8 @@ static int rope_bridge_run(void* qkv, int64_t ld, const void* tb, int64_t ldt, c
     if (positions && pos_stride != 1 && pos_stride != 2) return LIBRA_ERR_SHAPE;
     if (H <= 0 || S <= 0 || S > max_pos || ld < 3 * H * 128 || ldt < 16 || ldc < H * 128) return LIBRA_ERR_SHAPE;
     if ((ld % 8) || (ldt % 8) || (ldc % 8)) return LIBRA_ERR_ALIGN;
-    if (!qkv || !tb || !bk_l || !bk_v || !bv_l || !bv_v || !flag || !cos || !sin || !k_cross || !v_cross) return LIBRA_ERR_ALIGN;
+    if (!qkv || !tb || !bk_l || !bk_v || !bv_l || !bv_v || !flag || !cos || !sin) return LIBRA_ERR_ALIGN;
+    if (!codes && (!k_cross || !v_cross)) return LIBRA_ERR_ALIGN;
     if (!al16(qkv) || !al16(tb) || !al16(bk_l) || !al16(bk_v) || !al16(bv_l) || !al16(bv_v) || !al16(cos) || !al16(sin) ||
         !al16(k_cross) || !al16(v_cross)) return LIBRA_ERR_ALIGN;
     RopeArgs a;
@@ -357,7 +413,9 @@ static int rope_bridge_run(void* qkv, int64_t ld, const void* tb, int64_t ldt, c
     a.tok = tok;
     const long gx = (N + tok * tpb - 1) / (tok * tpb), gy = LT >= 256 ? (LT + 255) / 256 : 1;
     if (gx > 0x7fffffffL || gy > 65535) return LIBRA_ERR_SHAPE;
-    hipLaunchKernelGGL(rope_bridge_kernel, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, (hipStream_t)stream, a);
+    a.codes = codes; a.scales = scales; a.cap = (int)capacity; a.lg = lg;
+    if (codes) hipLaunchKernelGGL(rope_bridge_kernel<true>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(rope_bridge_kernel<false>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, (hipStream_t)stream, a);
     return launched();
 }
 
@@ -388,6 +446,21 @@ extern "C" int libra_rope_bridge_pos_append(void* qkv, int64_t ld, const void* t
     void* const cache[4] = {cache_k_same, cache_k_cross, cache_v_same, cache_v_cross};
     return rope_bridge_run(qkv, ld, tb, ldt, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, max_pos, k_cross, v_cross, ldc, B, max_pos, H,
                            positions, pos_stride, stream, cache, row_stride, batch_stride, slot);
+}
+
+extern "C" int libra_kv8_geometry_(const void* codes, const void* scales, int64_t B, int64_t H, int64_t capacity, int64_t block);
+
+extern "C" int libra_rope_bridge_pos_append8(void* qkv, int64_t ld, const void* tb, int64_t ldt, const void* bk_l, const void* bk_v,
+                                             const void* bv_l, const void* bv_v, const uint8_t* flag, const void* cos, const void* sin,
+                                             int64_t max_pos, int64_t B, const int* positions, int64_t pos_stride, int64_t H,
+                                             uint8_t* codes, uint8_t* scales, int64_t capacity, int64_t block, const int64_t* slot,
+                                             void* stream) {
+    if (B == 0) return LIBRA_OK;
+    const int lg = libra_kv8_geometry_(codes, scales, B, H, capacity, block);
+    if (lg < 0) return lg;
+    if (!positions || !slot) return LIBRA_ERR_ALIGN;
+    return rope_bridge_run(qkv, ld, tb, ldt, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, max_pos, nullptr, nullptr, H * 128, B, max_pos, H,
+                           positions, pos_stride, stream, nullptr, 0, 0, slot, codes, scales, capacity, lg);
 }
 
 extern "C" int libra_swiglu(const void* gate, const void* up, int64_t ldgu, void* y, int64_t ldy, int64_t rows,

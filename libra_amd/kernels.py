@@ -1070,6 +1070,28 @@ def kv8_append(rows, codes: torch.Tensor, scales: torch.Tensor, slot: torch.Tens
     _lib.check(rc, "kv8_append")
 
 
+def rope_bridge_pos_append8(qkv, tb, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, positions, H: int, codes: torch.Tensor, scales: torch.Tensor,
+                            slot: torch.Tensor) -> None:
+    """A generation step's rope_bridge_pos with an 8-bit cache: q and K_same rotated in place, the four rows of every new token (row n =
+    sequence n) quantised into slot `slot` (cuda int64 [1]) in the same launch - rope_bridge_pos followed by kv8_append, bit for bit."""
+    B, Hc, cap, block = _kv8_geometry(codes, scales, "rope_bridge_pos_append8")
+    _chk2d(qkv, "qkv"); _chk2d(tb, "tb")
+    if qkv.shape[0] != B or tb.shape[0] != B or Hc != H or qkv.shape[1] != 3 * H * 128:
+        raise ValueError(f"rope_bridge_pos_append8: qkv must be [{B}, {3 * Hc * 128}] for this cache, got {tuple(qkv.shape)}")
+    if positions.dtype != torch.int32 or positions.numel() not in (B, 2 * B) or not positions.is_contiguous():
+        raise ValueError("rope_bridge_pos_append8: positions must be contiguous int32 [B] or [B, 2]")
+    if slot.dtype != torch.int64 or slot.numel() != 1:
+        raise ValueError("rope_bridge_pos_append8: slot must be a cuda int64 tensor with one element")
+    if B == 0:
+        return
+    _here("rope_bridge_pos_append8", qkv, tb, flag, positions, codes, scales, slot)
+    rc = _lib.lib().libra_rope_bridge_pos_append8(qkv.data_ptr(), qkv.stride(0), tb.data_ptr(), tb.stride(0), bk_l.data_ptr(),
+                                                  bk_v.data_ptr(), bv_l.data_ptr(), bv_v.data_ptr(), flag.data_ptr(), cos.data_ptr(),
+                                                  sin.data_ptr(), cos.shape[0], B, positions.data_ptr(), positions.numel() // B, H,
+                                                  codes.data_ptr(), scales.data_ptr(), cap, block, slot.data_ptr(), _stream())
+    _lib.check(rc, "rope_bridge_pos_append8")
+
+
 def kv8_read(codes: torch.Tensor, scales: torch.Tensor, first: int, n: int, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Tokens [first, first + n) as bf16 rows [4, B, n, H*128] (K_same, K_cross, V_same, V_cross) - exactly what the cache stands for."""
     B, H, cap, block = _kv8_geometry(codes, scales, "kv8_read")

@@ -270,6 +270,32 @@ def test_captured_step_replays(K):
     assert all(torch.equal(c[0], caches[0][0]) and torch.equal(c[1], caches[0][1]) for c in caches[1:])
 
 
+@pytest.mark.parametrize("B,H,block,two", [(3, 2, 16, False), (8, 32, 16, True), (1, 5, 64, False), (2, 17, 1, True)])
+def test_rope_append_is_rope_then_append(K, B, H, block, two):
+    """The fused step == rope_bridge_pos followed by kv8_append, bit for bit, token by token over block borders."""
+    from oracle import libra_oracle as LO
+    D, cap = H * 128, 64
+    cosf, sinf = LO.rope_tables(128, 64)
+    cos, sin = cosf.to(BF).cuda(), sinf.to(BF).cuda()
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    w = [0.3 * rnd(D, 8) for _ in range(4)]
+    a, b = K.kv8_alloc(B, cap, H, "cuda", block), K.kv8_alloc(B, cap, H, "cuda", block)
+    for t in list(range(19)) + [63, 64]:                # (64: outside, stores nothing)
+        flag = (torch.rand(B, generator=g) < 0.5).to(torch.uint8).cuda()
+        pos = torch.randint(0, 64, (B, 2) if two else (B,), generator=g).to(torch.int32).cuda()
+        tb = torch.zeros(B, 64, dtype=BF, device="cuda"); tb[:, :16] = rnd(B, 16)
+        qkv = (rnd(B, 3 * D + 64) * (1 + t % 5))[:, :3 * D]
+        q2 = qkv.clone()
+        slot = torch.tensor([t], device="cuda")
+        K.rope_bridge_pos_append8(qkv, tb, *w, flag, cos, sin, pos, H, *a, slot)
+        kc, vc = K.rope_bridge_pos(q2, tb, *w, flag, cos, sin, pos, H)
+        K.kv8_append((q2[:, D:2 * D], kc, q2[:, 2 * D:], vc), *b, slot)
+        assert torch.equal(qkv, q2) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), t
+    with pytest.raises(ValueError):
+        K.rope_bridge_pos_append8(qkv, tb, *w, flag, cos, sin, pos, H + 1, *a, slot)
+
+
 def test_other_stream(K):
     """Work enqueued on a side stream runs on that stream."""
     q, codes, scales, g = attn_case(K, 2, 4, 256, 16, 12)
