@@ -347,18 +347,63 @@ class KVCache:
     """Per-layer key / value cache of the generation path (the reference's 4-tuple ([K_for_vision, K_for_language], V,
     V_bridge, vision_flag), modeling_libra.py:344-361), held as the four row buffers the kernels produce anyway:
     K_same = rope(k), K_cross = rope(k + kb), V_same = v, V_cross = v + vb, each [B, capacity, H] bf16, plus the modality
-    flag [B, capacity] of every cached token.  `length` tokens are valid in every sequence (no padding inside the cache)."""
+    flag [B, capacity] of every cached token.  `length` tokens are valid in every sequence (no padding inside the cache).
 
-    def __init__(self, layers: int, B: int, capacity: int, H: int, device):
+    dtype "fp8": the same rows in one byte a value (K.kv8_alloc: e4m3 codes, one power-of-two scale for every `block` tokens and head) -
+    half the memory and half the bytes of a step's attention; a cached value is off by at most half an e4m3 step.  The prompt's own
+    attention runs on the exact rows; what later steps read of it is quantised."""
+
+    def __init__(self, layers: int, B: int, capacity: int, H: int, device, *, dtype: str = "bf16", block: int = K.KV8_BLOCK):
+        if dtype not in ("bf16", "fp8"):
+            raise ValueError(f"KV cache dtype must be 'bf16' or 'fp8', got {dtype!r}")
         self.B, self.capacity, self.length = B, capacity, 0
-        self.layers = [tuple(torch.empty((B, capacity, H), dtype=BF16, device=device) for _ in range(4)) for _ in range(layers)]
-        self.flag = torch.zeros((B, capacity), dtype=torch.uint8, device=device)
+        self.dtype = dtype
+        if dtype == "fp8":
+            self.layers = [K.kv8_alloc(B, capacity, H // 128, device, block) for _ in range(layers)]           # (codes, scales)
+            slots = K.round_up(capacity, block)
+        else:
+            self.layers = [tuple(torch.empty((B, capacity, H), dtype=BF16, device=device) for _ in range(4)) for _ in range(layers)]
+            slots = capacity
+        self.flag = torch.zeros((B, slots), dtype=torch.uint8, device=device)
         self.start: Optional[torch.Tensor] = None          # int32 [B] first valid slot of each sequence (left-padded prompts)
         self.graphs: Dict[tuple, tuple] = {}               # routing pattern of a decode step -> (hipGraph, static buffers, outputs)
         self.pack_key = None                               # version of the packed weights the graphs were captured against
         self.sd = None                                     # the owner model's parameter dict at prefill (reused by its decode steps)
         self.run2d: Optional[torch.Tensor] = None          # use_2d_rope: int64 [B] running position (get_2d_position_ids' cumsum) at the last token
         self.hid: Optional[torch.Tensor] = None            # vision_prediction_mode="2d": final hidden state of every cached token [B, capacity, H]
+
+    def write_prompt(self, i: int, rows, S: int, starts: Optional[torch.Tensor] = None) -> None:
+        """Layer i's four row buffers [B*S, H] of a prompt into slots [0, S)."""
+        if self.dtype == "fp8":
+            K.kv8_fill(rows, *self.layers[i], S, kv_start=starts)
+        else:
+            for buf, r in zip(self.layers[i], rows):
+                buf[:, :S].copy_(r.view(self.B, S, -1))      # plumbing copies
+
+    def rows(self, i: int, first: int = 0, n: Optional[int] = None):
+        """Layer i's cached tokens [first, first + n) (default: all valid ones) as four bf16 tensors [B, n, H] (K_same, K_cross, V_same,
+        V_cross): the values that attention reads."""
+        n = self.length - first if n is None else n
+        if first < 0 or n < 0 or first + n > self.length:
+            raise ValueError(f"tokens [{first}, {first + n}) of a cache that holds {self.length}")
+        if self.dtype == "fp8":
+            return tuple(K.kv8_read(*self.layers[i], first, n))
+        return tuple(t[:, first:first + n] for t in self.layers[i])
+
+    def reorder(self, beam_idx: torch.Tensor) -> None:
+        """Re-gather the batch dimension (beam search, modeling_libra.py:1284-1289)."""
+        dim = 1 if self.dtype == "fp8" else 0
+        self.layers = [tuple(t.index_select(dim, beam_idx) for t in layer) for layer in self.layers]
+        self.flag = self.flag.index_select(0, beam_idx)
+        for nm in ("start", "run2d", "hid"):
+            t = getattr(self, nm)
+            if t is not None:
+                setattr(self, nm, t.index_select(0, beam_idx))
+        self.B = int(beam_idx.numel())
+        self.graphs.clear()                                  # captured steps point at the buffers just replaced
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for layer in self.layers for t in layer)
 
     def get_seq_length(self) -> int:
         return self.length
@@ -431,23 +476,30 @@ def layer_forward(sd, pk, i: int, d: DecDims, x, flag, lang_idx, vis_idx, lens, 
             K.gemm_nt_grouped([t[:, j * r:(j + 1) * r] for j in range(3)],
                               [sd[a + f"vision_{nm}_proj.weight_B"] for nm in ("q", "k", "v")],
                               [qkv[:, j * H:(j + 1) * H] for j in range(3)], c_rows=vis_idx)
+    q8 = cache is not None and cache.dtype == "fp8"
     fused_append = cache is not None and slot is not None and positions is not None
+    bridge = (qkv, tb, pk["bk_l"], pk["bk_v"], pk["bv_l"], pk["bv_v"], flag, cos, sin)
     if positions is None:
-        kc, vc = K.rope_bridge(qkv, tb, pk["bk_l"], pk["bk_v"], pk["bv_l"], pk["bv_v"], flag, cos, sin, S, d.heads)
+        kc, vc = K.rope_bridge(*bridge, S, d.heads)
+    elif fused_append and q8:
+        K.rope_bridge_pos_append8(*bridge, positions, d.heads, *cache.layers[i], slot)
     else:                                                   # (decode step: the new token's four cache rows go out of the same launch)
-        kc, vc = K.rope_bridge_pos(qkv, tb, pk["bk_l"], pk["bk_v"], pk["bv_l"], pk["bv_v"], flag, cos, sin, positions, d.heads,
-                                   append=(cache.layers[i], slot) if fused_append else None)
-    if cache is not None:                                   # the cache slots
+        kc, vc = K.rope_bridge_pos(*bridge, positions, d.heads, append=(cache.layers[i], slot) if fused_append else None)
+    if cache is not None and not fused_append:              # the cache slots
         new_rows = (qkv[:, H:2 * H], kc, qkv[:, 2 * H:], vc)
         if slot is None:
-            for buf, rows in zip(cache.layers[i], new_rows):
-                buf[:, :S].copy_(rows.view(B, S, H))         # prefill: plumbing copies
-        elif not fused_append:
+            cache.write_prompt(i, new_rows, S, kv_start)
+        elif q8:
+            K.kv8_append(new_rows, *cache.layers[i], slot)
+        else:
             K.kv_cache_append(new_rows, cache.layers[i], slot)
     if slot is None:
         o_lo = torch.empty((N, H), dtype=BF16, device=dev) if save else None   # rounding residual of o (the backward's D = dO.O)
         o, lse = K.bridge_attn_fwd(qkv[:, :H], qkv[:, H:2 * H], kc, qkv[:, 2 * H:], vc, flag, lens, B, S, d.heads,
                                    (H // d.heads) ** -0.5, need_lse=save, kv_start=kv_start, out_lo=o_lo)
+    elif q8:
+        o_lo = lse = None
+        o = K.bridge_attn_decode8(qkv[:, :H], *cache.layers[i], cache.flag, flag, lens, (H // d.heads) ** -0.5, kv_start=kv_start)
     else:
         ks_c, kc_c, vs_c, vc_c = cache.layers[i]
         o_lo = None
@@ -581,12 +633,13 @@ def heads_forward(sd, d: DecDims, hidden, flag, lang_idx, vis_idx, Q: int, *, un
 
 def forward(sd, packed, d: DecDims, input_ids, attention_mask, vision_indices, signal, labels=None, *,
             want_hidden_states: bool = False, save: bool = False, cache: Optional[KVCache] = None,
-            recompute: bool = False, inputs_embeds: Optional[torch.Tensor] = None):
+            recompute: bool = False, inputs_embeds: Optional[torch.Tensor] = None, score: Optional[int] = None):
     """-> dict(hidden [B,S,H], flag, lang_idx, vis_idx, z_lang [n_l,V], z_vis list of [n_v,Vv], loss or None, saved).
     `inputs_embeds` [B,S,H] with input_ids None (LibraModel.forward, modeling_libra.py:703-716, :748-754): the decoder runs on the
     given embeddings - no table lookup, no signal processing (upstream applies both only when it computes the embeddings itself);
     backward() then leaves the gradient w.r.t. them in out["d_inputs_embeds"].
     `cache` (empty KVCache): prefill - every layer's K/V rows of the prompt are stored for decode_step.
+    `score` (with labels): instead of the loss, out["scores"] = score_heads(...) with that many alternatives a position.
     `recompute` (with save): gradient checkpointing per decoder layer (modeling_libra.py:787-797) - only each layer's
     INPUT is kept; backward() re-runs layer_forward before layer_backward (4.3 GB instead of 61 GB at B=8, S=2048)."""
     if (input_ids is None) == (inputs_embeds is None):
@@ -625,7 +678,7 @@ def forward(sd, packed, d: DecDims, input_ids, attention_mask, vision_indices, s
             row = torch.where((vl >= 1) & (vl <= d.max_vision_len - 2), cell // d.res + 1, torch.zeros_like(vl))
             cache.run2d = pos2[:, -1, 0].long() - row
     # the loss's per-codebook target counts (shifted labels >= 0) are known before the first layer: read with the id check
-    cnts = [(labels[q][:, 1:] >= 0).sum().clamp_min(1) for q in range(Q)] if labels is not None else []
+    cnts = [(labels[q][:, 1:] >= 0).sum().clamp_min(1) for q in range(Q)] if labels is not None and score is None else []
     if input_ids is not None:
         counts = check_ids(input_ids, flag.view(B, S).bool(), d, also=cnts)
     else:
@@ -678,9 +731,11 @@ def forward(sd, packed, d: DecDims, input_ids, attention_mask, vision_indices, s
             K.copy_rows(hidden_src, src2d[0], n_v, feats, 0)
             K.copy_rows(hidden_src, src2d[1], n_v, feats, d.hidden)
     z_lang, z_vis, z_all = heads_forward(sd, d, hidden, flag, lang_idx, vis_idx, Q, unified=unified, feats=feats, packed=packed)
-    loss = None
+    loss = scores = None
     tgts = []
-    if labels is not None:
+    if score is not None:
+        scores = score_heads(d, labels, z_lang, z_vis, z_all, lang_idx, vis_idx, score)
+    elif labels is not None:
         loss = torch.zeros((), dtype=torch.float32, device=dev)
         for q in range(Q):
             tgt = torch.full((B, S), -100, dtype=torch.int64, device=dev)
@@ -703,9 +758,51 @@ def forward(sd, packed, d: DecDims, input_ids, attention_mask, vision_indices, s
     if save:
         saved.update(x_last=x, rstd_f=rstd_f, hidden=hidden, tgts=tgts, counts=counts, cos=cos, sin=sin, lens=lens, B=B, S=S,
                      Q=Q, input_ids=input_ids, positions=positions, unified=unified, src2d=src2d, feats=feats,
-                     vision_indices=vision_indices)
+                     vision_indices=vision_indices, scores=scores)
     return dict(hidden=hidden.view(B, S, d.hidden), flag=flag, lang_idx=lang_idx, vis_idx=vis_idx, z_lang=z_lang,
-                z_vis=z_vis, z_all=z_all, loss=loss, hidden_states=hs, saved=saved)
+                z_vis=z_vis, z_all=z_all, loss=loss, hidden_states=hs, saved=saved, scores=scores)
+
+
+def score_heads(d: DecDims, labels, z_lang, z_vis, z_all, lang_idx, vis_idx, top: int):
+    """Log probability of labels [Q, B, S] (< 0: not scored) under the model, entropy and `top` alternatives, each at the position of
+    the token it is about (position t: predicted by the row of token t - 1; position 0 is predicted by nothing):
+    logprobs, entropy fp32 [Q, B, S] (0 where not scored), top_ids int64 / top_logprobs fp32 [Q, B, S, top] (-1 / -inf at position 0).
+    Every head is read once: a text row answers for all codebooks (one distribution, Q given tokens).  `parts` is what the backward
+    takes: (which head, its logits, targets, first id, stats), rows in head order."""
+    Q, B, S = labels.shape
+    N, dev = B * S, labels.device
+    tgt = torch.full((Q, B, S), -100, dtype=torch.int64, device=dev)
+    tgt[:, :, :-1] = labels[:, :, 1:]                                              # the row of token t - 1 predicts token t
+    tgt = tgt.view(Q, N)
+    lp, ent = torch.zeros((Q, N), dtype=torch.float32, device=dev), torch.zeros((Q, N), dtype=torch.float32, device=dev)
+    ids = torch.full((Q, N, top), -1, dtype=torch.int64, device=dev)
+    tlp = torch.full((Q, N, top), float("-inf"), dtype=torch.float32, device=dev)
+    parts = []
+
+    def head(which, z, qs, rows, sub):
+        t = tgt[qs].contiguous() if rows is None else tgt[qs].index_select(1, rows).contiguous()
+        r = K.token_logprobs(z, t, target_sub=sub, top=top)
+        for j, q in enumerate(range(Q)[qs]):
+            at = slice(None) if rows is None else rows
+            lp[q, at], ent[q, at] = r.logprobs[j], r.entropy
+            ids[q, at], tlp[q, at] = r.top_ids, r.top_logprobs
+        parts.append((which, z, t, sub, r.stats))
+    if z_all is not None:
+        for q in range(Q):
+            head(("all", q), z_all[q], slice(q, q + 1), None, 0)
+    else:
+        if z_lang is not None:
+            head(("lang", None), z_lang, slice(0, Q), lang_idx.long(), 0)
+        for q in range(Q):
+            if z_vis[q] is not None:
+                head(("vis", q), z_vis[q], slice(q, q + 1), vis_idx.long(), d.vocab)
+    scored = (tgt >= 0).float()
+
+    def shift(x, first):                                                            # row of token t - 1 -> position t
+        x = x.view(Q, B, S, *x.shape[2:])
+        return torch.cat([torch.full_like(x[:, :, :1], first), x[:, :, :-1]], 2)
+    return dict(logprobs=shift(lp, 0), entropy=shift(ent * scored, 0), top_ids=shift(ids, -1), top_logprobs=shift(tlp, float("-inf")),
+                parts=parts, scored=scored)
 
 
 def _decode_core(sd, packed, d: DecDims, cache: KVCache, st: dict):
@@ -905,8 +1002,9 @@ def _norm_wgrad(dy, x, rstd, flag, lang_idx, vis_idx, want_l: bool, want_v: bool
     return out[:H], out[H:]
 
 
-def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
+def backward(sd, packed, d: DecDims, out, want, gscale=1.0, g_scores=None):
     """Gradients of out["loss"] w.r.t. every parameter name in `want` (a set) -> {name: bf16 grad}.
+    g_scores (a forward with `score`): (gradient of logprobs, gradient of entropy), fp32 [Q, B, S] at the positions of score_heads.
     gscale: the upstream gradient of the loss - a float, or a one-element device tensor (autograd's incoming scalar), which is
     applied inside the logits-gradient kernel and never read by the host."""
     sv = out["saved"]
@@ -926,7 +1024,13 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
     gdev = None
     if isinstance(gscale, torch.Tensor):
         gdev, gscale = gscale.detach().reshape(1).to(device=dev, dtype=torch.float32), 1.0
-    coef = [float(gscale / (sv["counts"][q] * Q)) for q in range(Q)]       # upstream gradient folded into dlogits
+    if g_scores is None:
+        coef = [float(gscale / (sv["counts"][q] * Q)) for q in range(Q)]   # upstream gradient folded into dlogits
+    else:
+        sc = {which: rest for which, *rest in sv["scores"]["parts"]}
+        # back to the rows that predict: position t -> the row of token t - 1 (the last row predicts nothing)
+        g_lp, g_en = (torch.cat([x[:, :, 1:], torch.zeros_like(x[:, :, :1])], 2).reshape(Q, N).contiguous() for x in g_scores)
+        g_en = g_en * sv["scores"]["scored"]
     def head_pad(name):
         """Head weight with its vocab (the dgrad reduction length) zero-padded to the GEMM's 64 granule."""
         W = sd[name]
@@ -938,10 +1042,23 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
         wp[:V] = W
         return wp, V, Vp
 
-    def dlogits(z, t0, t1, sub, c0, c1, Vp):
+    def dlogits(which, q, Vp):
+        """Gradient of the logits of a head ("lang": text rows, all codebooks; "vis" / "all": codebook q), zero pad rows AND columns."""
+        z = out["z_lang"] if which == "lang" else out["z_vis" if which == "vis" else "z_all"][q]
         n, V = z.shape
-        full = torch.zeros((K.round_up(n, 64), Vp), dtype=BF16, device=dev)      # zero pad rows AND pad columns
-        K.ce_rows_bwd(z, t0, t1, sub, c0, c1, full[:n, :V], scale=gdev)
+        full = torch.zeros((K.round_up(n, 64), Vp), dtype=BF16, device=dev)
+        if g_scores is not None:
+            _, t, sub, stats = sc[(which, q)]
+            qs = slice(0, Q) if which == "lang" else slice(q, q + 1)
+            at = None if which == "all" else (lang_idx if which == "lang" else vis_idx).long()
+            gl, ge = (x[qs] if at is None else x[qs].index_select(1, at) for x in (g_lp, g_en))
+            K.token_logprobs_bwd(z, t, stats, gl.contiguous(), ge.sum(0), target_sub=sub, out=full[:n, :V])
+        elif which == "lang":
+            t = [sv["tgts"][k][0] for k in range(Q)]
+            K.ce_rows_bwd(z, t[0], t[1] if Q > 1 else None, 0, coef[0], coef[1] if Q > 1 else 0.0, full[:n, :V], scale=gdev)
+        else:
+            sub = d.vocab if which == "vis" else 0
+            K.ce_rows_bwd(z, sv["tgts"][q][1 if which == "vis" else 0], None, sub, coef[q], 0.0, full[:n, :V], scale=gdev)
         return full
 
     if Q > 2:
@@ -955,7 +1072,7 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
         for q in range(Q):
             name = f"vision_lm_head.heads.{q}.weight"
             wcat = packed.heads[q]                                       # [Vp, H]: the forward's operand, pad rows zero
-            dzf = dlogits(out["z_all"][q], sv["tgts"][q][0], None, 0, coef[q], 0.0, Vp)
+            dzf = dlogits("all", q, Vp)
             K.gemm_nt(dzf[:N], wcat, b_t=True, out=dhid, resid=dhid if q > 0 else None)
             if w(name) or w("lm_head.weight"):
                 gw = K.gemm_nt(dzf, _full(hid_c), a_t=True, b_t=True)
@@ -966,9 +1083,8 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
         if gl is not None:
             g["lm_head.weight"] = gl.to(BF16)
     if n_l and not sv["unified"]:
-        tl = [sv["tgts"][q][0] for q in range(Q)]
         wl, V, Vp = head_pad("lm_head.weight")
-        dzf = dlogits(out["z_lang"], tl[0], tl[1] if Q > 1 else None, 0, coef[0], coef[1] if Q > 1 else 0.0, Vp)
+        dzf = dlogits("lang", None, Vp)
         K.gemm_nt(dzf[:n_l], wl, b_t=True, out=dhid, c_rows=lang_idx)
         if w("lm_head.weight"):
             g["lm_head.weight"] = K.gemm_nt(dzf, _full(_compact(hidden, lang_idx)), a_t=True, b_t=True)[:V]
@@ -977,7 +1093,7 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
         for q in range(Q):
             name = f"vision_lm_head.heads.{q}.weight"
             wq, V, Vp = head_pad(name)
-            dzf = dlogits(out["z_vis"][q], sv["tgts"][q][1], None, d.vocab, coef[q], 0.0, Vp)
+            dzf = dlogits("vis", q, Vp)
             K.gemm_nt(dzf[:n_v], wq, b_t=True, out=dhid, c_rows=vis_idx, resid=dhid if q > 0 else None)
             if w(name):
                 hv = _compact(hidden, vis_idx) if hv is None else hv
@@ -989,7 +1105,7 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0):
         for q in range(Q):
             name = f"vision_lm_head.heads.{q}.weight"
             wq, V, Vp = head_pad(name)
-            dzf = dlogits(out["z_vis"][q], sv["tgts"][q][1], None, d.vocab, coef[q], 0.0, Vp)
+            dzf = dlogits("vis", q, Vp)
             K.gemm_nt(dzf[:n_v], wq, b_t=True, out=dfeat, resid=dfeat if q > 0 else None)
             if w(name):
                 g[name] = K.gemm_nt(dzf, _full(feats), a_t=True, b_t=True)[:V]

@@ -16,6 +16,8 @@ from typing import Callable, List, Optional, Sequence, Tuple, Union
 import torch
 from transformers.utils import ModelOutput
 
+from .. import kernels as K
+
 
 class ValidImageLogitsProcessor:
     """Keeps a generated image well-formed: once a BOI has been emitted, exactly `valid_image_token_length` code tokens follow
@@ -86,6 +88,11 @@ class LibraGenerateOutput(ModelOutput):
     sequences: torch.LongTensor = None                      # [Q, B, S_total]
     scores: Optional[Tuple[torch.FloatTensor]] = None       # per step [Q, B, V + Vv] (processed)
     logits: Optional[Tuple[torch.FloatTensor]] = None       # per step, raw
+    # output_logprobs: about every generated token under the distribution it was chosen from (after processors and warpers)
+    logprobs: Optional[torch.FloatTensor] = None            # [Q, B, T] (0 for the padding behind a finished sequence)
+    entropy: Optional[torch.FloatTensor] = None             # [Q, B, T] (the same)
+    top_ids: Optional[torch.LongTensor] = None              # [Q, B, T, top_logprobs] most likely ids, equal ones by the smaller id
+    top_logprobs: Optional[torch.FloatTensor] = None        # [Q, B, T, top_logprobs]
 
 
 def _run_all(fns, input_ids, scores):
@@ -105,7 +112,8 @@ class LibraGenerationMixin:
     def _generation_loop(self, input_ids, choose: Callable, *, logits_processor=None, logits_warper=None, stopping_criteria=None,
                          max_length: Optional[int] = None, pad_token_id: Optional[int] = None,
                          eos_token_id: Optional[Union[int, Sequence[int]]] = None, output_scores: bool = False,
-                         output_logits: bool = False, return_dict_in_generate: bool = False, streamer=None, **model_kwargs):
+                         output_logits: bool = False, return_dict_in_generate: bool = False, streamer=None,
+                         output_logprobs: bool = False, top_logprobs: int = 0, **model_kwargs):
         if input_ids.dim() != 3:
             raise ValueError("input_ids must be [Q, B, S] (one row of ids per codebook)")
         cfg = self.config
@@ -122,7 +130,9 @@ class LibraGenerationMixin:
         model_kwargs.setdefault("use_cache", True)
         if max_length is not None:
             model_kwargs.setdefault("max_cache_len", max_length)      # sizes the KV cache (instead of max_position_embeddings)
-        scores_t, logits_t = [], []
+        scores_t, logits_t, scored_t = [], [], []
+        if top_logprobs and not output_logprobs:
+            raise ValueError("top_logprobs needs output_logprobs=True")
 
         def stop(ids0) -> bool:
             if max_length is not None and ids0.shape[-1] >= max_length:
@@ -136,8 +146,8 @@ class LibraGenerationMixin:
             model_inputs = self.prepare_inputs_for_generation(input_ids, **model_kwargs)
             model_inputs.pop("past_hidden_states", None)
             model_inputs.pop("past_vision_flag", None)
-            max_cache_len = model_kwargs.get("max_cache_len")
-            outputs = self(**model_inputs, return_dict=True, **({"max_cache_len": max_cache_len} if max_cache_len else {}))
+            cache_kw = {k: model_kwargs[k] for k in ("max_cache_len", "cache_dtype", "cache_block") if model_kwargs.get(k)}
+            outputs = self(**model_inputs, return_dict=True, **cache_kw)
             raw = outputs.logits[:, :, -1, :]
             nxt_scores = _run_all(logits_warper, input_ids, _run_all(logits_processor, input_ids, raw))
             if output_scores:
@@ -145,15 +155,19 @@ class LibraGenerationMixin:
             if output_logits:
                 logits_t.append(raw)
             next_tokens = choose(nxt_scores)                             # [Q, B]
-            cols = []
+            cols, given = [], []
             for q in range(input_ids.shape[0]):                          # codebook by codebook, like the reference: a sequence that
                 tok = next_tokens[q]                                     # ends in codebook q is already padded in codebook q + 1
+                if output_logprobs:
+                    given.append(torch.where(unfinished > 0, tok, torch.full_like(tok, -100)))
                 if eos is not None:
                     tok = tok * unfinished + pad_token_id * (1 - unfinished)
                     unfinished = unfinished * (tok[None, :] != eos[:, None]).all(0).long()
                 if streamer is not None:
                     streamer.put(tok.cpu())
                 cols.append(tok)
+            if output_logprobs:
+                scored_t.append(self._score_step(nxt_scores, torch.stack(given), top_logprobs))
             model_kwargs = self._update_model_kwargs_for_generation(outputs, model_kwargs)
             input_ids = torch.cat([input_ids, torch.stack(cols)[:, :, None]], dim=-1)
             done = eos is not None and int(unfinished.max()) == 0
@@ -162,23 +176,39 @@ class LibraGenerationMixin:
         if streamer is not None:
             streamer.end()
         if return_dict_in_generate:
+            scored = [torch.stack(x, 2) for x in zip(*scored_t)] if output_logprobs else [None] * 4
             return LibraGenerateOutput(sequences=input_ids, scores=tuple(scores_t) if output_scores else None,
-                                       logits=tuple(logits_t) if output_logits else None)
+                                       logits=tuple(logits_t) if output_logits else None, logprobs=scored[0], entropy=scored[1],
+                                       top_ids=scored[2] if top_logprobs else None, top_logprobs=scored[3] if top_logprobs else None)
         return input_ids
+
+    @staticmethod
+    def _score_step(scores: torch.Tensor, given: torch.Tensor, top: int):
+        """scores [Q, B, V'] and the chosen tokens [Q, B] (-100: a finished sequence's padding) -> their log probability, the entropy
+        [Q, B] (0 behind a sequence's end) and the most likely ids with theirs [Q, B, top]: one launch for all codebooks."""
+        Q, B, V = scores.shape
+        z = scores.reshape(Q * B, V)
+        if z.dtype not in (torch.bfloat16, torch.float32):
+            z = z.float()
+        r = K.token_logprobs(z, given.reshape(1, Q * B).contiguous(), top=top)
+        return (r.logprobs.view(Q, B), torch.where(given >= 0, r.entropy.view(Q, B), torch.zeros_like(r.entropy.view(Q, B))),
+                r.top_ids.view(Q, B, top), r.top_logprobs.view(Q, B, top))
 
     @torch.no_grad()
     def greedy_search(self, input_ids, logits_processor=None, stopping_criteria=None, max_length=None, pad_token_id=None,
-                      eos_token_id=None, output_scores=False, return_dict_in_generate=False, streamer=None, **model_kwargs):
+                      eos_token_id=None, output_scores=False, return_dict_in_generate=False, streamer=None, output_logprobs=False,
+                      top_logprobs=0, **model_kwargs):
         """argmax per codebook and sequence (modeling_libra_utils.py:61-328)."""
         return self._generation_loop(input_ids, lambda s: torch.argmax(s, dim=-1), logits_processor=logits_processor,
                                      stopping_criteria=stopping_criteria, max_length=max_length, pad_token_id=pad_token_id,
                                      eos_token_id=eos_token_id, output_scores=output_scores,
-                                     return_dict_in_generate=return_dict_in_generate, streamer=streamer, **model_kwargs)
+                                     return_dict_in_generate=return_dict_in_generate, streamer=streamer,
+                                     output_logprobs=output_logprobs, top_logprobs=top_logprobs, **model_kwargs)
 
     @torch.no_grad()
     def sample(self, input_ids, logits_processor=None, stopping_criteria=None, logits_warper=None, max_length=None,
                pad_token_id=None, eos_token_id=None, output_scores=False, output_logits=False, return_dict_in_generate=False,
-               streamer=None, generator: Optional[torch.Generator] = None, **model_kwargs):
+               streamer=None, generator: Optional[torch.Generator] = None, output_logprobs=False, top_logprobs=0, **model_kwargs):
         """one multinomial draw per codebook and sequence from softmax(scores) (modeling_libra_utils.py:330-620)."""
         def choose(scores):
             # a forced token is scored +inf (the EOI -> newline rule): clamp so that its probability is 1, not NaN
@@ -187,13 +217,16 @@ class LibraGenerationMixin:
         return self._generation_loop(input_ids, choose, logits_processor=logits_processor, logits_warper=logits_warper,
                                      stopping_criteria=stopping_criteria, max_length=max_length, pad_token_id=pad_token_id,
                                      eos_token_id=eos_token_id, output_scores=output_scores, output_logits=output_logits,
-                                     return_dict_in_generate=return_dict_in_generate, streamer=streamer, **model_kwargs)
+                                     return_dict_in_generate=return_dict_in_generate, streamer=streamer,
+                                     output_logprobs=output_logprobs, top_logprobs=top_logprobs, **model_kwargs)
 
     @torch.no_grad()
     def generate(self, input_ids, *, attention_mask=None, vision_indices=None, contiguous_signal=None, max_new_tokens: int = 20,
                  max_length: Optional[int] = None, do_sample: bool = False, temperature: float = 1.0, top_k: int = 0,
                  logits_processor=None, **kwargs):
-        """Convenience front end: greedy (default) or temperature / top-k sampling until `max_length` / EOS."""
+        """Convenience front end: greedy (default) or temperature / top-k sampling until `max_length` / EOS.
+        cache_dtype="fp8" (with cache_block=16): the KV cache in 8 bits.  return_dict_in_generate=True with output_logprobs=True,
+        top_logprobs=k: log probability, entropy and the k most likely ids of every generated position."""
         if attention_mask is None:
             attention_mask = torch.ones(input_ids.shape[1:], dtype=torch.long, device=input_ids.device)
         if vision_indices is None:

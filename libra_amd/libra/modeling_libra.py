@@ -19,6 +19,7 @@ import torch
 from torch import nn
 from transformers import PreTrainedModel
 from transformers.modeling_outputs import CausalLMOutputWithPast
+from transformers.utils import ModelOutput
 
 from .. import decoder_engine as DE
 from ..common.registry import registry
@@ -153,6 +154,16 @@ class LibraCausalLMOutputWithPast(CausalLMOutputWithPast):     # modeling_libra.
         return super().__getitem__(k)
 
 
+@dataclass
+class LibraTokenLogprobs(ModelOutput):
+    """LibraForCausalLM.token_logprobs: everything about the token AT its position t (predicted from the tokens before it).
+    logprobs, entropy fp32 [Q, B, S] (0 where not scored; with a gradient), top_ids int64 / top_logprobs fp32 [Q, B, S, top]."""
+    logprobs: Optional[torch.FloatTensor] = None
+    entropy: Optional[torch.FloatTensor] = None
+    top_ids: Optional[torch.LongTensor] = None
+    top_logprobs: Optional[torch.FloatTensor] = None
+
+
 class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
     config_class = LibraConfig
     base_model_prefix = "model"
@@ -277,7 +288,8 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
                 position_ids=None, past_key_values=None, inputs_embeds=None, labels: Optional[torch.LongTensor] = None,
                 use_cache: Optional[bool] = None, output_attentions=None, output_hidden_states=None, return_dict=None,
                 contiguous_signal: Optional[torch.Tensor] = None, vision_indices: Optional[torch.LongTensor] = None,
-                past_hidden_states=None, past_vision_flag=None, max_cache_len: Optional[int] = None):
+                past_hidden_states=None, past_vision_flag=None, max_cache_len: Optional[int] = None, cache_dtype: Optional[str] = None,
+                cache_block: Optional[int] = None):
         if input_ids is not None and inputs_embeds is not None:                        # modeling_libra.py:703-704
             raise ValueError("You cannot specify both decoder_input_ids and decoder_inputs_embeds at the same time")
         if input_ids is None and inputs_embeds is None:                                # :715-716
@@ -297,7 +309,7 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
             if labels is not None:
                 raise ValueError("labels with use_cache / past_key_values: the cached path is inference only (:1142)")
             return self._forward_cached(input_ids, attention_mask, position_ids, past_key_values, contiguous_signal, vision_indices,
-                                        max_cache_len)
+                                        max_cache_len, cache_dtype, cache_block)
         if position_ids is not None:
             raise NotImplementedError("custom position_ids on the training path (positions are arange(S), :736-739)")
         B, S = lead.shape[1:3] if input_ids is not None else lead.shape[:2]
@@ -324,14 +336,46 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
         res.__dict__["_engine_out"] = out
         return res
 
+    def token_logprobs(self, input_ids: torch.LongTensor, labels: Optional[torch.LongTensor] = None, *,
+                       attention_mask: Optional[torch.Tensor] = None, vision_indices: Optional[torch.LongTensor] = None,
+                       contiguous_signal: Optional[torch.Tensor] = None, top: int = 0) -> LibraTokenLogprobs:
+        """Score given tokens: log probability of labels [Q, B, S] (default: the input ids themselves where attention_mask allows;
+        < 0: not scored) under the uncached forward, with each predicting distribution's entropy and its `top` (<= 64) most likely ids.
+        logprobs and entropy carry a gradient to the parameters - the losses that `labels=` of forward() does not cover (a reward- or
+        preference-weighted log likelihood, an entropy bonus) are ordinary expressions of them."""
+        if vision_indices is None:
+            raise ValueError("You have to specify vision_indices [B,S] (the modality of every position, :1116)")
+        if not input_ids.is_cuda:
+            raise RuntimeError("libra_amd LibraForCausalLM runs on MI355X only; got CPU tensors (no CPU fallback)")
+        if input_ids.dim() != 3 or len(input_ids) != self.config.vision_codebook_num:
+            raise ValueError(f"input_ids must be [{self.config.vision_codebook_num}, B, S], got {tuple(input_ids.shape)}")
+        Q, B, S = input_ids.shape
+        limit = min(64, self.config.vocab_size, self.config.vision_vocab_size)
+        if not 0 <= top <= limit:
+            raise ValueError(f"top must be 0..{limit}, got {top}")
+        if attention_mask is None:
+            attention_mask = torch.ones((B, S), dtype=torch.bool, device=input_ids.device)
+        if labels is None:
+            labels = input_ids.masked_fill(attention_mask[None] == 0, -100)
+        if tuple(labels.shape) != (Q, B, S) or labels.dtype != torch.int64:
+            raise ValueError(f"labels must be int64 {(Q, B, S)}, got {labels.dtype} {tuple(labels.shape)}")
+        names, params = self._named_params()
+        holder = {"grad_on": torch.is_grad_enabled()}
+        lp, ent = _LibraScoreFunction.apply(self, holder, names, input_ids, attention_mask, vision_indices, contiguous_signal, labels, int(top),
+                                            *params)
+        return LibraTokenLogprobs(logprobs=lp, entropy=ent, top_ids=holder["top_ids"], top_logprobs=holder["top_logprobs"])
+
     @torch.no_grad()
-    def _forward_cached(self, input_ids, attention_mask, position_ids, past, signal, vision_indices, max_cache_len=None):
+    def _forward_cached(self, input_ids, attention_mask, position_ids, past, signal, vision_indices, max_cache_len=None,
+                        cache_dtype=None, cache_block=None):
         """Generation path (LibraForCausalLM.forward with use_cache / past_key_values, modeling_libra.py:1118-1188):
         `past` None = prefill of the prompt (returns a filled DE.KVCache as `.past_key_values`); otherwise one new token per
         sequence.  Batched prompts are padded on the LEFT (positions = attention_mask.cumsum - 1, :1204-1207; pad keys are
         masked by the kernels through the cache's per-sequence start).  `.logits` is materialised ([Q,B,q,V+Vv], q = the tokens
         of this call) with the cached branch's rule that an EOI input token predicts nothing but a newline (:1141-1144).
-        The KV cache holds `max_cache_len` tokens (default max_position_embeddings; generate() passes its max_length)."""
+        The KV cache holds `max_cache_len` tokens (default max_position_embeddings; generate() passes its max_length), as bf16 rows or
+        with cache_dtype="fp8" in 8 bits (a scale for every `cache_block` tokens and head, default 16): half the memory and half the bytes
+        a step reads of it.  Both are chosen by the call that prefills; later steps go by the cache they are given."""
         Q, B, S = input_ids.shape
         dims = self._dims
         # A decode step continues the generation its prefill started: the operand copies were checked and refreshed there, and
@@ -356,7 +400,8 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
                 if not torch.equal(position_ids.reshape(B, S).to(dev), want):
                     raise NotImplementedError("prefill positions other than attention_mask.cumsum(-1) - 1")
             cap = max(int(max_cache_len), S + 1) if max_cache_len else max(dims.max_pos, S + 1)
-            cache = DE.KVCache(dims.layers, B, cap, dims.hidden, dev)
+            cache = DE.KVCache(dims.layers, B, cap, dims.hidden, dev, dtype=cache_dtype or "bf16",
+                               **({"block": cache_block} if cache_block is not None else {}))
             cache.pack_key = ptr_key
             cache.sd = sd
             out = DE.forward(sd, packed, dims, input_ids, attention_mask, vision_indices, signal, None, cache=cache)
@@ -437,14 +482,7 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
     @staticmethod
     def _reorder_cache(past_key_values, beam_idx):
         """modeling_libra.py:1284-1289 for the KVCache container (beam search re-gathers the batch dimension)."""
-        past_key_values.layers = [tuple(t.index_select(0, beam_idx) for t in layer) for layer in past_key_values.layers]
-        past_key_values.flag = past_key_values.flag.index_select(0, beam_idx)
-        for nm in ("start", "run2d", "hid"):
-            t = getattr(past_key_values, nm, None)
-            if t is not None:
-                setattr(past_key_values, nm, t.index_select(0, beam_idx))
-        past_key_values.B = int(beam_idx.numel())
-        past_key_values.graphs.clear()                                   # captured steps point at the buffers just replaced
+        past_key_values.reorder(beam_idx)
         return past_key_values
 
     @staticmethod
@@ -491,6 +529,37 @@ class _LibraFunction(torch.autograd.Function):
         d_emb = ctx.out.pop("d_inputs_embeds", None)
         d_emb = d_emb.to(ctx.embeds_dtype) if (d_emb is not None and ctx.embeds_dtype is not None) else None
         return (None,) * 9 + (d_emb,) + tuple(res)
+
+
+class _LibraScoreFunction(torch.autograd.Function):
+    """LibraForCausalLM.token_logprobs as an autograd node: forward = DE.forward(score=...), backward = DE.backward from the gradients of
+    logprobs and entropy.  Parameter gradients as in _LibraFunction."""
+
+    @staticmethod
+    def forward(ctx, model, holder, names, input_ids, attention_mask, vision_indices, signal, labels, top, *params):
+        sd = dict(zip(names, params))
+        packed = model._refresh_packed(sd)
+        need = holder["grad_on"] and any(ctx.needs_input_grad[9:])
+        out = DE.forward(sd, packed, model._dims, input_ids, attention_mask, vision_indices, signal, labels, save=need,
+                         recompute=need and model.model.gradient_checkpointing and model.training, score=top)
+        sc = out["scores"]
+        holder["top_ids"], holder["top_logprobs"] = sc["top_ids"], sc["top_logprobs"]
+        ctx.model, ctx.sd, ctx.out, ctx.names = model, sd, out, names
+        ctx.want = {n for n, ng in zip(names, ctx.needs_input_grad[9:]) if ng}
+        return sc["logprobs"], sc["entropy"]
+
+    @staticmethod
+    def backward(ctx, g_lp, g_ent):
+        if ctx.out.get("saved") is None:
+            raise RuntimeError("backward through token_logprobs requested but no activations were saved (or it ran already)")
+        grads = DE.backward(ctx.sd, ctx.model._packed, ctx.model._dims, ctx.out, ctx.want, g_scores=(g_lp.float(), g_ent.float()))
+        from .. import dp
+        res = []
+        for n in ctx.names:
+            gr = grads.get(n) if n in ctx.want and not dp.is_captured(n) else None      # captured: lives in the DP bucket
+            res.append(gr.reshape(ctx.sd[n].shape) if gr is not None else None)
+        ctx.out["saved"] = None
+        return (None,) * 9 + tuple(res)
 
 
 def _cfg_get(cfg, key, default=None):

@@ -69,6 +69,54 @@ def test_c_entry_points_refuse(L):
         assert attn(**bad) == ERR_ALIGN, bad
 
 
+    def rope(**kw):
+        a = dict(dict(qkv=FAKE, ld=768, tb=FAKE, ldt=64, kl=FAKE, kv=FAKE, vl=FAKE, vv=FAKE, flag=FAKE, cos=FAKE, sin=FAKE, mp=64, B=2, pos=FAKE, ps=1,
+                      H=2, codes=FAKE, scales=FAKE, cap=32, block=16, slot=FAKE, st=None), **kw)
+        return L.libra_rope_bridge_pos_append8(*a.values())
+    assert rope(B=0) == OK
+    for bad in (dict(ld=512), dict(ldt=8), dict(ps=3), dict(cap=33), dict(block=6), dict(mp=0), dict(B=-2)):
+        assert rope(**bad) == ERR_SHAPE, bad
+    for bad in (dict(pos=None), dict(slot=None), dict(codes=None), dict(qkv=P(0x10008)), dict(cos=None), dict(ld=769)):
+        assert rope(**bad) == ERR_ALIGN, bad
+
+
+def test_log_probability_entry_points_refuse(L):
+    def fwd(**kw):
+        a = dict(dict(z=FAKE, ldz=100, rows=4, V=100, f32=0, t=FAKE, T=2, sub=0, lp=FAKE, st=FAKE, top=3, ids=FAKE, tlp=FAKE, s=None), **kw)
+        return L.libra_token_logprobs(*a.values())
+    assert fwd(rows=0) == OK
+    for bad in (dict(V=0), dict(ldz=99), dict(T=65), dict(T=-1), dict(top=65), dict(top=101, V=100), dict(top=-1), dict(rows=-1)):
+        assert fwd(**bad) == ERR_SHAPE, bad
+    for bad in (dict(z=None), dict(z=P(0x10001)), dict(z=P(0x10002), f32=1), dict(t=None), dict(lp=None), dict(st=None), dict(ids=None), dict(tlp=None)):
+        assert fwd(**bad) == ERR_ALIGN, bad
+
+    def bwd(**kw):
+        a = dict(dict(z=FAKE, ldz=100, rows=4, V=100, f32=0, t=FAKE, T=2, sub=0, st=FAKE, g=FAKE, ge=None, dz=FAKE, lddz=100, s=None), **kw)
+        return L.libra_token_logprobs_bwd(*a.values())
+    assert bwd(rows=0) == OK
+    assert bwd(lddz=99) == ERR_SHAPE and bwd(V=0) == ERR_SHAPE
+    for bad in (dict(dz=None), dict(dz=P(0x10001)), dict(st=None), dict(t=None), dict(z=None)):
+        assert bwd(**bad) == ERR_ALIGN, bad
+
+
+def test_cache_container_on_the_host():
+    """KVCache dtype "fp8": buffers, capacity rounding, batch re-gather - no kernel involved."""
+    from libra_amd import decoder_engine as DE
+    c = DE.KVCache(3, 2, 21, 512, "cpu", dtype="fp8", block=16)
+    assert len(c.layers) == 3 and tuple(c.layers[0][0].shape) == (4, 2, 4, 32, 128) and tuple(c.flag.shape) == (2, 32) and c.capacity == 21
+    for i, (codes, scales) in enumerate(c.layers):
+        codes.copy_(torch.arange(2, dtype=torch.uint8)[None, :, None, None, None].expand_as(codes) + i)
+    c.start, c.graphs = torch.tensor([3, 5], dtype=torch.int32), {"x": 1}
+    c.reorder(torch.tensor([1, 1, 0]))
+    assert c.B == 3 and c.start.tolist() == [5, 5, 3] and not c.graphs
+    assert [int(c.layers[2][0][0, b, 0, 0, 0]) for b in range(3)] == [3, 3, 2] and tuple(c.layers[0][1].shape) == (4, 3, 4, 2)
+    assert c.nbytes() * 2 < DE.KVCache(3, 3, 32, 512, "cpu").nbytes() * 1.01
+    with pytest.raises(ValueError):
+        DE.KVCache(1, 1, 8, 128, "cpu", dtype="int8")
+    with pytest.raises(ValueError):
+        c.rows(0, 0, 1)
+
+
 def test_host_wrappers_refuse_without_a_gpu():
     """Shapes, types and devices are judged before anything is launched."""
     from libra_amd import kernels as K

@@ -8,6 +8,7 @@ from libra_amd.libra import LibraConfig, LibraForCausalLM
 B = int(sys.argv[1]) if len(sys.argv) > 1 else 8
 P = int(sys.argv[2]) if len(sys.argv) > 2 else 1024
 STEPS = int(sys.argv[3]) if len(sys.argv) > 3 else 32
+CACHE = sys.argv[4] if len(sys.argv) > 4 else "bf16"            # "bf16" or "fp8"
 dev = torch.device("cuda")
 cfg = LibraConfig()
 with torch.device(dev):
@@ -33,7 +34,7 @@ sig[:, 2:L] = torch.randn(B, L - 2, cfg.contiguous_signal_size, generator=g).to(
 ids, vi, sig = ids.to(dev), vi.to(dev), sig.to(dev)
 with torch.no_grad():
     torch.cuda.synchronize(); t0 = time.perf_counter()
-    out = m(input_ids=ids, vision_indices=vi, contiguous_signal=sig, use_cache=True)
+    out = m(input_ids=ids, vision_indices=vi, contiguous_signal=sig, use_cache=True, max_cache_len=P + STEPS + 8, cache_dtype=CACHE)
     torch.cuda.synchronize(); t_pre = time.perf_counter() - t0
     past = out.past_key_values
     nxt = out.logits[0, :, -1, :V].argmax(-1)
@@ -48,6 +49,6 @@ with torch.no_grad():
         tok = out.logits[0, :, -1, :V].argmax(-1); tok = torch.stack([tok, tok])[:, :, None]
     torch.cuda.synchronize(); dt = (time.perf_counter() - t0) / STEPS
 nparam = sum(p.numel() for n, p in m.named_parameters() if "vision" not in n) * 2
-print(f"B={B} prompt={P}: prefill {t_pre * 1e3:.1f} ms (first call, includes operand packing); decode {dt * 1e3:.2f} ms/step = "
+print(f"B={B} prompt={P} cache={CACHE} {past.nbytes() / 1e9:.1f} GB: prefill {t_pre * 1e3:.1f} ms (first call, includes operand packing); decode {dt * 1e3:.2f} ms/step = "
       f"{B / dt:.0f} tokens/s; text-weight bytes per step {nparam / 1e9:.1f} GB -> {nparam / dt / 1e12:.2f} TB/s effective; "
       f"cache length {past.get_seq_length()}")
