@@ -1,6 +1,6 @@
 // Log probabilities of given tokens, entropy and the largest alternatives of a row of logits z[V] (bf16 or fp32), and the gradient.
-//   m = max z,  e_v = exp(z_v - m),  r = sum of e over every column but ONE that attains m (so r is exact to fp32 relative precision
-//   also where one token is nearly certain),  log p_v = (z_v - m) - log1p(r),  H = log1p(r) - sum e_v (z_v - m) / (1 + r)
+//   m = max z,  e_v = exp(z_v - m),  r = sum of e over every column but ONE that attains m (so r has fp32's relative precision also
+//   where one token is nearly certain),  log p_v = (z_v - m) - log1p(r),  H = log1p(r) - sum e_v (z_v - m) / (1 + r)
 // (both terms of H are >= 0: no cancellation).  A row whose maximum is +inf (a forced token) is shared by its n infinite columns:
 // log p = -log n there, -inf elsewhere, H = log n - the formulas as they stand with z_v - m := 0 where z_v = m.  A row of nothing but
 // -inf answers log p = -inf, H = 0.  A row that holds a NaN answers NaN.
@@ -37,8 +37,8 @@ template <> struct LpElem<float> {
     static __device__ __forceinline__ u32x4 pack_all(float v) { const unsigned w = __float_as_uint(v); return u32x4{w, w, w, w}; }
 };
 // A row is read in 16-byte pieces, piece c = the columns [c VEC, (c + 1) VEC), wherever the row begins (any V, any row stride: the
-// hardware loads 16 bytes at any address of the element's alignment).  The last, partial piece is cut out of the row's last 16 bytes:
-// nothing outside the row is read.  Columns behind the row's end come as -inf.
+// hardware loads 16 bytes at any address of the element's alignment); the fewer than VEC columns behind the last whole piece are
+// taken one a thread.  Nothing outside the row is read.
 template <typename T>
 __device__ __forceinline__ u32x4 lp_whole(const T* at) {
     u32x4 q;
@@ -46,31 +46,14 @@ __device__ __forceinline__ u32x4 lp_whole(const T* at) {
     return q;
 }
 template <typename T>
-__device__ __forceinline__ u32x4 lp_tail(const T* row, int V, int c) {
-    constexpr int VEC = LpElem<T>::VEC;
-    const int v0 = c * VEC;
-    if (V < VEC) {
-        float f[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = v0 + e < V ? LpElem<T>::get(row[v0 + e]) : -INFINITY;
-        return LpElem<T>::pack(f);
-    }
-    const u32x4 q = lp_whole(row + V - VEC), none = LpElem<T>::pack_all(-INFINITY);
-    const int s = (v0 + VEC - V) * (int)sizeof(T) * 8;               // bits that belong to the piece before: shifted out
-    unsigned long long lo = q[0] | (unsigned long long)q[1] << 32, hi = q[2] | (unsigned long long)q[3] << 32, mlo = ~0ull, mhi = ~0ull;
-    if (s >= 64) { lo = hi; mlo = mhi; hi = mhi = 0; }
-    const int r = s & 63;
-    if (r) {
-        lo = lo >> r | hi << (64 - r); hi >>= r;
-        mlo = mlo >> r | mhi << (64 - r); mhi >>= r;
-    }
-    return u32x4{(unsigned)lo | (none[0] & ~(unsigned)mlo), (unsigned)(lo >> 32) | (none[1] & ~(unsigned)(mlo >> 32)),
-                 (unsigned)hi | (none[2] & ~(unsigned)mhi), (unsigned)(hi >> 32) | (none[3] & ~(unsigned)(mhi >> 32))};
-}
-template <typename T>
 __device__ __forceinline__ void lp_load(const T* row, int V, int c, float* f) {
     constexpr int VEC = LpElem<T>::VEC;
-    LpElem<T>::unpack((c + 1) * VEC <= V ? lp_whole(row + c * VEC) : c * VEC < V ? lp_tail(row, V, c) : LpElem<T>::pack_all(-INFINITY), f);
+    if ((c + 1) * VEC <= V) {
+        LpElem<T>::unpack(lp_whole(row + c * VEC), f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = c * VEC + e < V ? LpElem<T>::get(row[c * VEC + e]) : -INFINITY;
+    }
 }
 // order of the alternatives: larger value first, then smaller column; NaN behind everything
 __device__ __forceinline__ unsigned long long lp_key(float z, int v) {
@@ -119,12 +102,13 @@ template <typename T, int NT, int NCH, bool TOP, int ROWS>
 __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_row_kernel(const LogprobArgs p) {
     static_assert(ROWS == 1 || (NT == 64 && !TOP), "several rows a workgroup: a wave each, nothing shared");
     typedef LpElem<T> E;
-    constexpr int VEC = E::VEC, NW = NT / 64, NV = NCH * VEC, NEAR = TOP ? 64 : 1, LIST = NEAR * NV;
+    constexpr int VEC = E::VEC, NW = NT / 64, NV = NCH * VEC, NEAR = TOP ? 64 : 1, LIST = NEAR * (NV + 1);
     constexpr int LOW = sizeof(T) == 2 ? 16 : 0;                     // lowest bit of the keys that tells two values apart
-    __shared__ float red_m[NW], red_s[NW], red_t[NW];
+    __shared__ float red_m[NW], red_s[NW], red_t[NW], red_e[NW];
     __shared__ unsigned keymax[TOP ? NT : 1];
     __shared__ u32x4 near_z[TOP ? NEAR * NCH : 1];                   // [NEAR][NCH] pieces of the threads that reach tau, and who they are
     __shared__ int near_tid[NEAR];
+    __shared__ float near_one[NEAR];
     __shared__ unsigned long long list[TOP ? LIST : 1];
     __shared__ unsigned nnear, nlist, tau_s, many_s, wtot[NW];
     const long row = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x >> 6 : 0);
@@ -132,17 +116,13 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
     const T* z = (const T*)p.z + row * p.ldz;
     const int tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x, wave = tid >> 6, lane = tid & 63;
     u32x4 raw[NCH];
-    const int whole = p.V / VEC;                                     // pieces 0 ... whole - 1 are whole, piece `whole` may be partial
+    const int whole = p.V / VEC, rest = whole * VEC;                 // whole pieces; thread t also holds column rest + t, if there is one
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         raw[i] = E::pack_all(-INFINITY);
         if (i * NT + tid < whole) raw[i] = lp_whole(z + (i * NT + tid) * VEC);
     }
-    if (whole * VEC < p.V && tid == whole % NT) {
-        const u32x4 part = lp_tail(z, p.V, whole);
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) if (i == whole / NT) raw[i] = part;
-    }
+    const float one = rest + tid < p.V ? E::get(z[rest + tid]) : -INFINITY;
     // the given tokens' logits: requested before the row's own reductions
     float zt = 0.f;
     long long tg = -1, tcol = -1;
@@ -152,7 +132,7 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         if (tg >= 0 && tcol >= 0 && tcol < p.V) zt = E::get(z[tcol]);
     }
     if (TOP && tid == 0) nnear = nlist = 0;
-    float mine = -INFINITY;
+    float mine = fmaxf(one, -INFINITY);                              // (a NaN does not count)
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         float f[VEC];
@@ -162,7 +142,8 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         __builtin_amdgcn_sched_barrier(0);
     }
     if (TOP) keymax[tid] = lp_sort(mine);
-    float m = lp_wave_max(mine);
+    const float mw = lp_wave_max(mine);
+    float m = mw;
     if (ROWS == 1) {
         if (lane == 0) red_m[wave] = m;
         __syncthreads();
@@ -170,47 +151,67 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
         for (int w = 0; w < NW; ++w) m = fmaxf(m, red_m[w]);
     }
     // (the floats are derived from the packed pieces anew in every phase: kept, they are twice the registers and half the waves)
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) pin(raw[i]);
-    // s = sum of 2^x, t = sum of 2^x x with x = z log2 e - c, c = m log2 e as rounded: one fused operation a column.  What c's rounding and
-    // log2 e's are off by is a factor common to all columns; it goes out with e_m = 2^x at z = m, by which r and the entropy divide.
-    // (c's rounding stays below 2^-9 for |m| < 16384; beyond that, and for infinite m, x = (z - m) log2 e.)
+    // s = sum of 2^x, t = sum of 2^x x over the columns BELOW m, eq = how many attain it; x = z log2 e - c, c = m log2 e as rounded: one fused
+    // operation a column.  What c's rounding and log2 e's are off by is a factor common to all columns; it goes out with em = 2^xm, xm =
+    // x at z = m.  (c's rounding stays below 2^-9 for |m| < 16384; beyond that, and for infinite m, x = (z - m) log2 e, xm = 0.)
+    // Only the wave that holds m has columns to leave out: the others take the short loop.
     constexpr float L2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
     const float c = m * L2E;
     const bool close = fabsf(m) < 16384.f;
-    float s = 0.f, t = 0.f;
-    if (close) {
+    float s, t, eq;
+    auto add = [&](float zv) {
+        const float x = close ? fmaf(zv, L2E, -c) : lp_diff(zv, m) * L2E, ex = zv == m ? 0.f : __builtin_amdgcn_exp2f(x);
+        eq += zv == m ? 1.f : 0.f;
+        s += ex;                                                     // (NaN iff the row has one)
+        t = fmaf(ex, fmaxf(x, -1e4f), t);                            // (2^x is 0 by then: keeps 0 * -inf out)
+    };
+    s = t = eq = 0.f;
+    add(one);
+    if (close && mw < m) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             float f[VEC];
+            pin(raw[i]);
             E::unpack(raw[i], f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float x = fmaf(f[e], L2E, -c);
-                const float ex = __builtin_amdgcn_exp2f(x);
-                s += ex;                                             // (NaN iff the row has one)
-                t = fmaf(ex, fmaxf(x, -1e4f), t);                    // (2^x is 0 by then: keeps 0 * -inf out)
+                const float x = fmaf(f[e], L2E, -c), ex = __builtin_amdgcn_exp2f(x);
+                s += ex;
+                t = fmaf(ex, fmaxf(x, -1e4f), t);
             }
             __builtin_amdgcn_sched_barrier(0);                       // (one piece at a time: 64 exponentials in flight double the registers)
         }
-    } else {                                                         // (forced rows, whose infinite columns share them, among these)
+    } else if (close) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             float f[VEC];
+            pin(raw[i]);
             E::unpack(raw[i], f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float x = lp_diff(f[e], m) * L2E;
-                const float ex = __builtin_amdgcn_exp2f(x);
+                const float x = fmaf(f[e], L2E, -c), ex = f[e] == m ? 0.f : __builtin_amdgcn_exp2f(x);
+                eq += f[e] == m ? 1.f : 0.f;
                 s += ex;
                 t = fmaf(ex, fmaxf(x, -1e4f), t);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        eq = lp_wave_sum(eq);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            float f[VEC];
+            pin(raw[i]);
+            E::unpack(raw[i], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) add(f[e]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        eq = lp_wave_sum(eq);
     }
     s = lp_wave_sum(s);
     t = lp_wave_sum(t);
-    if (ROWS == 1 && lane == 0) { red_s[wave] = s; red_t[wave] = t; }
+    if (ROWS == 1 && lane == 0) { red_s[wave] = s; red_t[wave] = t; red_e[wave] = mw < m ? 0.f : eq; }
     if (TOP && wave == 0) {                                          // tau, by wave 0
         unsigned key[NW];
 #pragma unroll
@@ -232,56 +233,18 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
     }
     if (ROWS == 1) {
         __syncthreads();
-        s = t = 0.f;
+        s = t = eq = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { s += red_s[w]; t += red_t[w]; }
-    }
-    const bool nan = s != s, empty = m == -INFINITY;
-    float xm = close ? fmaf(m, L2E, -c) : 0.f, em = __builtin_amdgcn_exp2f(xm);
-    float r = s - em;
-    if (r < 0.125f && !empty && !nan) {
-        // one column holds nearly everything: the others by themselves, from z - m (differences of sums near 1 would lose them)
-        float eq = 0.f;
-        s = t = 0.f;
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) pin(raw[i]);
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            float f[VEC];
-            E::unpack(raw[i], f);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const bool at = f[e] == m;
-                const float x = fmaxf((f[e] - m) * L2E, -1e4f), ex = at ? 0.f : __builtin_amdgcn_exp2f(x);
-                eq += at ? 1.f : 0.f;
-                s += ex;
-                t += at ? 0.f : ex * x;
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        s = lp_wave_sum(s);
-        t = lp_wave_sum(t);
-        eq = lp_wave_sum(eq);
-        if (ROWS == 1) {
-            __syncthreads();                                         // (uniform: every thread has the same r; the old sums are read)
-            if (lane == 0) { red_s[wave] = s; red_t[wave] = t; red_m[wave] = eq; }
-            __syncthreads();
-            s = t = eq = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) { eq += red_m[w]; s += red_s[w]; t += red_t[w]; }
-        }
-        r = (eq - 1.f) + s;
-        s += eq;
-        em = 1.f;
-        xm = 0.f;
+        for (int w = 0; w < NW; ++w) { s += red_s[w]; t += red_t[w]; eq += red_e[w]; }
     }
     if (!TOP && wave > 0) return;                                    // (what is left is a few numbers a row)
-    const bool sure = r < 0.125f;
-    r *= __builtin_amdgcn_rcpf(em);                                  // sum of exp(z - m) beside one column that attains m
+    const bool nan = s != s, empty = m == -INFINITY;
+    const float xm = close ? fmaf(m, L2E, -c) : 0.f, iem = __builtin_amdgcn_exp2f(-xm);
+    const float r = (eq - 1.f) + s * iem;                            // sum of exp(z - m) beside one column that attains m
     const float qnan = __uint_as_float(0x7fc00000u);
-    // H = log1p(r) - sum p (z - m), sum p (z - m) = ln 2 (t - xm s) / s
-    const float lsum = empty ? 0.f : sure ? log1pf(r) : __builtin_amdgcn_logf(1.f + r) * LN2;
-    const float ent = empty ? 0.f : lsum - LN2 * (t - xm * s) * __builtin_amdgcn_rcpf(s);
+    const float lsum = empty ? 0.f : r < 0.125f ? log1pf(r) : __builtin_amdgcn_logf(1.f + r) * LN2;
+    // H = log1p(r) - sum p (z - m); the columns at m have no part in the second sum
+    const float ent = empty ? 0.f : lsum - LN2 * (t - xm * s) * iem * __builtin_amdgcn_rcpf(1.f + r);
     auto logp = [&](float zv) { return nan ? qnan : empty ? -INFINITY : lp_diff(zv, m) - lsum; };
     if (tid == 0) {
         p.stats[row] = nan ? qnan : m;
@@ -296,6 +259,7 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
             const unsigned at = atomicAdd(&nnear, 1u);
             if (at < NEAR) {
                 near_tid[at] = tid;
+                near_one[at] = one;
 #pragma unroll
                 for (int i = 0; i < NCH; ++i) near_z[at * NCH + i] = raw[i];
             }
@@ -307,24 +271,29 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
             const int v = (i * NT + near_tid[at]) * VEC + e;
             const unsigned long long key = lp_key(E::get(((const T*)near_z)[x]), v);
             const unsigned u = (unsigned)(key >> 32);
+            if (v < rest && (many ? u > tau : u >= tau)) list[atomicAdd(&nlist, 1u)] = key;
+        }
+        for (int x = tid; x < nn / NV; x += NT) {
+            const int v = rest + near_tid[x];
+            const unsigned long long key = lp_key(near_one[x], v);
+            const unsigned u = (unsigned)(key >> 32);
             if (v < p.V && (many ? u > tau : u >= tau)) list[atomicAdd(&nlist, 1u)] = key;
         }
         __syncthreads();
         int n = (int)nlist;
         int need = p.top - n;                                        // > 0 only where many: the first columns that equal tau fill up
         // (a thread without columns, or with NaNs only, counted as -inf above: where that made tau -inf, NaNs fill what is still missing)
-        for (int k = 0; k < 2 * NCH && need > 0; ++k) {              // (uniform; one pass nearly always, the others' pieces come from the cache)
-            const int i = k < NCH ? k : k - NCH;
-            const unsigned want = k < NCH ? tau : 0u;
+        for (int k = 0; k < 2 * (NCH + 1) && need > 0; ++k) {        // (uniform; one pass nearly always, the others' pieces come from the cache)
+            const int i = k <= NCH ? k : k - (NCH + 1);
+            const unsigned want = k <= NCH ? tau : 0u;
             float f[VEC];
+            int v0 = (i * NT + tid) * VEC, end = rest;
             if (i == 0) E::unpack(raw[0], f);
-            else lp_load(z, p.V, i * NT + tid, f);
+            else if (i < NCH) lp_load(z, p.V, i * NT + tid, f);
+            else { v0 = rest + tid; end = min(v0 + 1, p.V); f[0] = one; }            // the columns behind the last whole piece
             unsigned mask = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const int v = (i * NT + tid) * VEC + e;
-                mask |= (v < p.V && lp_sort(f[e]) == want) ? 1u << e : 0u;
-            }
+            for (int e = 0; e < VEC; ++e) mask |= (v0 + e < end && lp_sort(f[e]) == want) ? 1u << e : 0u;
             int incl = __popc(mask);
             for (int o = 1; o < 64; o <<= 1) { const int up = __shfl_up(incl, o, 64); incl += lane >= o ? up : 0; }
             if (lane == 63) wtot[wave] = (unsigned)incl;
@@ -335,7 +304,7 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 if (mask >> e & 1) {
-                    if (before < need) list[n + before] = lp_key(f[e], (i * NT + tid) * VEC + e);
+                    if (before < need) list[n + before] = lp_key(f[e], v0 + e);
                     ++before;
                 }
             const int got = total < need ? total : need;
@@ -493,6 +462,16 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
         }
     }
     const float ls2 = lsum * L2E, a0 = flat ? 0.f : g + gh * ent, a1 = flat ? 0.f : gh * LN2;
+    // a given token's column: its share as -expm1(log p) - 1 - p taken as a difference would lose a sure token's gradient
+    auto given = [&](float zv, long long tg) {
+        const float lp = zv - m - lsum, pr = __expf(lp), one = -expm1f(lp);
+        float sum = -(pr > 0.f ? pr * (lp + ent) * gh : 0.f);
+        for (int k = 0; k < p.T; ++k) {
+            const long long tk = p.targets[k * p.rows + row];
+            if (tk >= 0) sum += p.g_lp[k * p.rows + row] * (tk == tg ? one : -pr);
+        }
+        return sum;
+    };
     auto piece = [&](int c, int j, float* f) {
         const int v0 = c * VEC;
         float zk[VEC];
@@ -510,13 +489,7 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
                 float zv = 0.f;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) zv = v0 + e == v ? zk[e] : zv;
-                // its share as -expm1(log p): 1 - p taken as a difference would lose a sure token's gradient
-                const float lp = zv - m - lsum, pr = __expf(lp), one = -expm1f(lp);
-                float sum = -(pr > 0.f ? pr * (lp + ent) * gh : 0.f);
-                for (int k = 0; k < p.T; ++k) {
-                    const long long tk = p.targets[k * p.rows + row];
-                    if (tk >= 0) sum += p.g_lp[k * p.rows + row] * (tk == tg ? one : -pr);
-                }
+                const float sum = given(zv, tg);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) f[e] = (v0 + e == v) ? sum : f[e];
             }
@@ -540,17 +513,21 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
             __builtin_memcpy(dz + (c + u * NT) * VEC, &o, 16);
         }
     }
-    for (; c * VEC < p.V; c += NT, ++j) {
+    for (; c < whole; c += NT, ++j) {
         float f[VEC];
-        lp_load(z, p.V, c, f);
+        LpElem<T>::unpack(lp_whole(z + c * VEC), f);
         piece(c, j, f);
-        if (c < whole) {
-            const u32x4 o = LpElem<T>::pack(f);
-            __builtin_memcpy(dz + c * VEC, &o, 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) if (c * VEC + e < p.V) dz[c * VEC + e] = LpElem<T>::put(f[e]);
-        }
+        const u32x4 o = LpElem<T>::pack(f);
+        __builtin_memcpy(dz + c * VEC, &o, 16);
+    }
+    const int v = whole * VEC + tid;                                 // a column behind the last whole piece
+    if (v < p.V) {
+        const float zv = LpElem<T>::get(z[v]), x = fmaxf(fmaf(zv - m, L2E, -ls2), -1e4f);
+        float d = -__builtin_amdgcn_exp2f(x) * fmaf(a1, x, a0);
+        if (p.g_lp)
+            for (int i = 0; i < p.T; ++i)
+                if (p.targets[i * p.rows + row] >= 0 && p.targets[i * p.rows + row] - p.tsub == v) { d = given(zv, p.targets[i * p.rows + row]); break; }
+        dz[v] = LpElem<T>::put(flat ? 0.f : d);
     }
 }
 template <typename T>
@@ -569,11 +546,13 @@ static void lp_launch(const LogprobArgs& a, hipStream_t st) {
     constexpr int W = 8 / LpElem<T>::VEC;                            // pieces are half as wide in fp32
     constexpr int R = TOP ? 1 : 4;                                   // short rows: four waves, four rows a workgroup
     const dim3 g((unsigned)a.rows);
-    const int need = a.V;
-    if (need <= 1024) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP, R>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(64 * R), 0, st, a);
-    else if (need <= 8192) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP, 1>), g, dim3(256), 0, st, a);
-    else if (need <= 32768) hipLaunchKernelGGL((logprobs_row_kernel<T, 512, 8 * W, TOP, 1>), g, dim3(512), 0, st, a);
-    else if (need <= 65536) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 8 * W, TOP, 1>), g, dim3(1024), 0, st, a);
+    const int P = a.V / LpElem<T>::VEC;                              // whole pieces
+    const dim3 g4((unsigned)((a.rows + R - 1) / R)), t4(64 * R);
+    if (P <= 64 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, W, TOP, R>), g4, t4, 0, st, a);
+    else if (P <= 128 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP, R>), g4, t4, 0, st, a);
+    else if (P <= 1024 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP, 1>), g, dim3(256), 0, st, a);
+    else if (P <= 4096 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 512, 8 * W, TOP, 1>), g, dim3(512), 0, st, a);
+    else if (P <= 8192 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 1024, 8 * W, TOP, 1>), g, dim3(1024), 0, st, a);
     else hipLaunchKernelGGL(logprobs_kernel<T>, g, dim3(LP_THREADS), 0, st, a);
 }
 
