@@ -1004,10 +1004,9 @@ KV8_BLOCK = 16             # tokens that share a scale unless a caller chooses o
 
 def _here(what: str, *ts) -> None:
     """Every tensor on the current device: the kernels run on its current stream."""
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
-            raise ValueError(f"{what}: every tensor must be on the current device (cuda:{dev}), got one on {t.device}")
+    at = {t.get_device() for t in ts if t is not None}               # (-1: a host tensor)
+    if len(at) != 1 or -1 in at or torch._C._cuda_getDevice() not in at:
+        raise ValueError(f"{what}: every tensor must be on the current device, got {[str(t.device) for t in ts if t is not None]}")
 
 
 def kv8_alloc(B: int, capacity: int, heads: int, device, block: int = KV8_BLOCK):
@@ -1022,16 +1021,17 @@ def kv8_alloc(B: int, capacity: int, heads: int, device, block: int = KV8_BLOCK)
 
 def _kv8_geometry(codes: torch.Tensor, scales: torch.Tensor, what: str):
     """-> (B, H, capacity, block)"""
-    cs, ss = codes.shape, scales.shape
-    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or len(cs) != 5 or len(ss) != 4 or cs[0] != 4 or cs[4] != 128 \
-            or cs[:3] != ss[:3] or not codes.is_contiguous() or not scales.is_contiguous():
-        raise ValueError(f"{what}: the cache is contiguous uint8 codes [4, B, H, capacity, 128] and scales [4, B, H, capacity / block], got "
-                         f"{codes.dtype} {tuple(cs)} and {scales.dtype} {tuple(ss)}")
-    cap, n = cs[3], ss[3]
-    block = cap // n if n else 0
-    if block * n != cap or block < 1 or block > 64 or block & (block - 1):
-        raise ValueError(f"{what}: capacity {cap} over {n} scales is not a block of 1, 2, 4, ... 64 tokens")
-    return cs[1], cs[2], cap, block
+    cs, ss = tuple(codes.shape), tuple(scales.shape)
+    if codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(cs) == 5 and len(ss) == 4 and codes.is_contiguous() \
+            and scales.is_contiguous():
+        four, B, H, cap, width = cs
+        n = ss[3]
+        if four == 4 and width == 128 and ss[0] == 4 and ss[1] == B and ss[2] == H and n:
+            block = cap // n
+            if block * n == cap and 1 <= block <= 64 and not block & (block - 1):
+                return B, H, cap, block
+    raise ValueError(f"{what}: the cache is contiguous uint8 codes [4, B, H, capacity, 128] and scales [4, B, H, capacity / block], block 1, 2, 4 "
+                     f"... 64, got {codes.dtype} {cs} and {scales.dtype} {ss}")
 
 
 def _kv8_rows(rows, n: int, width: int, what: str):
@@ -1040,10 +1040,11 @@ def _kv8_rows(rows, n: int, width: int, what: str):
         raise ValueError(f"{what}: four row buffers (K_same, K_cross, V_same, V_cross) are expected, got {len(rows)}")
     args = []
     for r in rows:
-        _chk2d(r, what + " rows")
-        if r.shape != (n, width):
-            raise ValueError(f"{what}: rows must be [{n}, {width}], got {tuple(r.shape)}")
-        args += (r.data_ptr(), r.stride(0))
+        st = r.stride()
+        if r.dtype is not BF16 or tuple(r.shape) != (n, width) or st[1] != 1:
+            raise ValueError(f"{what}: rows must be row-major bf16 [{n}, {width}], got {r.dtype} {tuple(r.shape)} strides {st}")
+        args.append(r.data_ptr())
+        args.append(st[0])
     return args
 
 
