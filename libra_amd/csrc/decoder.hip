@@ -98,37 +98,38 @@ __device__ __forceinline__ u32x2 pack4(const float* f) {
     u32x2 v; v[0] = pack2bf(f[0], f[1]); v[1] = pack2bf(f[2], f[3]); return v;
 }
 
-// One row of one head into an 8-bit cache: the 16 lanes c of a head hold its channels [4c, 4c + 4) and [64 + 4c, 64 + 4c + 4) (x[0], x[1]).
-// The steps of kv8_append: a block's first token sets its scale, a later one that needs more re-expresses the block's earlier codes.
-__device__ __forceinline__ void rope_store8(const RopeArgs& p, int which, long n, int h, int c, int slot, const float (&x)[2][4]) {
-    unsigned mx = 0;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { const unsigned a = kv8_abs_bits(x[hf][e]); mx = a > mx ? a : mx; }
-    int byte = kv8_byte(row16_max(mx));
-    const long head = ((long)which * p.N + n) * p.H + h;
-    unsigned char* sc = p.scales + head * (p.cap >> p.lg) + (slot >> p.lg);
-    unsigned char* dst = p.codes + head * p.cap * 128 + c * 4;
+// One token's four rows of one head into an 8-bit cache: the 16 lanes c of a head hold the channels [4c, 4c + 4) and [64 + 4c, 64 + 4c + 4)
+// of each (x[0], x[1]); old = the four blocks' scale bytes.  The steps of kv8_append: a block's first token sets its scale, a later one that
+// needs more re-expresses the block's earlier codes (rare after a block's first tokens: one copy of that code, not four).
+__device__ __forceinline__ void rope_store8(const RopeArgs& p, long head, long plane, int c, int slot, const int (&old)[4],
+                                            const float (&x0)[2][4], const float (&x1)[2][4], const float (&x2)[2][4], const float (&x3)[2][4]) {
     const int in_block = slot & ((1 << p.lg) - 1);
-    if (in_block) {
-        const int old = min((int)sc[0], 254);
-        if (byte > old) {
-            const float down = kv8_scale(max(127 + old - byte, 0));
-            for (long t = slot - in_block; t < slot; ++t) {
-                unsigned* w = (unsigned*)(dst + t * 128);
-                w[0] = kv8_rescale4(w[0], down);
-                w[16] = kv8_rescale4(w[16], down);
-            }
-        } else {
-            byte = old;
-        }
+    unsigned char* codes = p.codes + head * p.cap * 128;
+    auto need_of = [](const float (&x)[2][4]) {
+        unsigned mx = 0;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const unsigned a = kv8_abs_bits(x[hf][e]); mx = a > mx ? a : mx; }
+        return kv8_byte(row16_max(mx));
+    };
+    const int n0 = need_of(x0), n1 = need_of(x1), n2 = need_of(x2), n3 = need_of(x3);
+    const int o0 = min(old[0], 254), o1 = min(old[1], 254), o2 = min(old[2], 254), o3 = min(old[3], 254);
+    if (in_block && (n0 > o0 || n1 > o1 || n2 > o2 || n3 > o3)) {
+#pragma unroll 1
+        for (int w = 0; w < 4; ++w)
+            kv8_grow(codes + (w * plane * p.cap + (slot - in_block)) * 128, in_block, w == 0 ? n0 : w == 1 ? n1 : w == 2 ? n2 : n3,
+                     w == 0 ? o0 : w == 1 ? o1 : w == 2 ? o2 : o3, c);
     }
-    const float inv = kv8_inverse(byte);
-    unsigned* w = (unsigned*)(dst + (long)slot * 128);
-    w[0] = kv8_encode4(x[0][0] * inv, x[0][1] * inv, x[0][2] * inv, x[0][3] * inv);
-    w[16] = kv8_encode4(x[1][0] * inv, x[1][1] * inv, x[1][2] * inv, x[1][3] * inv);
-    if (c == 0) sc[0] = (unsigned char)byte;
+    auto store = [&](int w, int need, int was, const float (&x)[2][4]) {
+        const int b = in_block ? max(need, was) : need;
+        const float inv = kv8_inverse(b);
+        unsigned* d = (unsigned*)(codes + (w * plane * p.cap + slot) * 128 + c * 4);
+        d[0] = kv8_encode4(x[0][0] * inv, x[0][1] * inv, x[0][2] * inv, x[0][3] * inv);
+        d[16] = kv8_encode4(x[1][0] * inv, x[1][1] * inv, x[1][2] * inv, x[1][3] * inv);
+        if (c == 0) p.scales[(head + w * plane) * (p.cap >> p.lg) + (slot >> p.lg)] = (unsigned char)b;
+    };
+    store(0, n0, o0, x0); store(1, n1, o1, x1); store(2, n2, o2, x2); store(3, n3, o3, x3);
 }
 
 template <bool Q8>
@@ -150,6 +151,19 @@ __global__ __launch_bounds__(256) void rope_bridge_kernel(const RopeArgs p) {
         while (s >= p.S) s -= p.S;
         const int pos = p.positions ? min(max(p.positions[n * p.pos_stride + (p.pos_stride == 2 ? (h & 1) : 0)], 0), p.max_pos - 1) : s;
         const int vis = p.flag[n] != 0;
+        // (8-bit cache: the four blocks' scales, requested ahead of everything that does not need them)
+        long long cslot = 0;
+        bool in_cache = false;
+        const long plane = p.N * p.H, head = n * p.H + h;
+        int old[4] = {0, 0, 0, 0};
+        if constexpr (Q8) {
+            cslot = p.slot[0];
+            in_cache = cslot >= 0 && cslot < p.cap;                   // outside: nothing is stored
+            if (in_cache) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) old[w] = p.scales[(head + w * plane) * (p.cap >> p.lg) + (cslot >> p.lg)];
+            }
+        }
         if (vis != cur_mod) {
             const bf16_t* bk = vis ? p.bk_v : p.bk_l;
             const bf16_t* bv = vis ? p.bv_v : p.bv_l;
@@ -208,12 +222,8 @@ __global__ __launch_bounds__(256) void rope_bridge_kernel(const RopeArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) vc[hf][e] = rbf(vc[hf][e]);
             }
-            const long long slot = p.slot[0];
-            if (slot >= 0 && slot < p.cap) {
-                rope_store8(p, 0, n, h, c, (int)slot, ko);
-                rope_store8(p, 1, n, h, c, (int)slot, kc);
-                rope_store8(p, 2, n, h, c, (int)slot, v);
-                rope_store8(p, 3, n, h, c, (int)slot, vc);
+            if (in_cache) {
+                rope_store8(p, head, plane, c, (int)cslot, old, ko, kc, v, vc);
             }
             continue;
         }

@@ -93,30 +93,18 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(const Kv8AppendArgs p) 
     if (h >= p.H || slot < 0 || slot >= p.cap) return;                // outside the cache: nothing is stored (as kv_cache_append)
     const bf16_t* src = w == 0 ? p.src[0] : w == 1 ? p.src[1] : w == 2 ? p.src[2] : p.src[3];
     const long ld = w == 0 ? p.ld[0] : w == 1 ? p.ld[1] : w == 2 ? p.ld[2] : p.ld[3];
+    const long head = ((long)w * p.B + b) * p.H + h;
+    unsigned char* sc = p.scales + head * (p.cap >> p.lg) + (slot >> p.lg);
+    const int old = sc[0];                                            // (in flight together with the row)
     float f[8];
     unpack8(*(const u32x4*)(src + b * ld + h * 128 + sub * 8), f);
     unsigned mx = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { const unsigned a = kv8_abs_bits(f[e]); mx = a > mx ? a : mx; }
     int byte = kv8_byte(row16_max(mx));
-    const long head = ((long)w * p.B + b) * p.H + h;
-    unsigned char* sc = p.scales + head * (p.cap >> p.lg) + (slot >> p.lg);
     unsigned char* dst = p.codes + head * p.cap * 128 + sub * 8;
     const int in_block = (int)slot & ((1 << p.lg) - 1);
-    if (in_block) {
-        const int old = min((int)sc[0], 254);
-        if (byte > old) {
-            const float down = kv8_scale(127 + old - byte > 0 ? 127 + old - byte : 0);
-            for (long t = slot - in_block; t < slot; ++t) {
-                u32x2 c = *(const u32x2*)(dst + t * 128);
-                c[0] = kv8_rescale4(c[0], down);
-                c[1] = kv8_rescale4(c[1], down);
-                *(u32x2*)(dst + t * 128) = c;
-            }
-        } else {
-            byte = old;
-        }
-    }
+    byte = kv8_grow(dst - sub * 8 + (slot - in_block) * 128, in_block, byte, old, sub);
     const float inv = kv8_inverse(byte);
     u32x2 c;
     c[0] = kv8_encode4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);

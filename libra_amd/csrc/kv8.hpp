@@ -44,11 +44,36 @@ __device__ __forceinline__ void kv8_decode4(unsigned w, float* f) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     f[0] = lo[0]; f[1] = lo[1]; f[2] = hi[0]; f[3] = hi[1];
 }
-// codes of a block whose scale grows by the factor 1 / down (down = 2^(old - new) < 1): exact but for values that leave the normal range
+// 4 codes of a block whose scale grows by the factor 1 / down (down = 2^(old - new) < 1): exact but for values that leave the normal range
 __device__ __forceinline__ unsigned kv8_rescale4(unsigned w, float down) {
     float f[4];
     kv8_decode4(w, f);
     return kv8_encode4(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
+}
+// The scale of a block that gets one more token (its `in_block`-th, 0 = the first; `need` = the byte that the token asks for, `old` = the
+// byte that was there): -> the byte to use; where it grows, the codes of the earlier tokens - `in_block` * 128 contiguous bytes at `codes` -
+// are re-expressed.  A 16-lane group does it (lane = 0..15), 16 tokens at a time with all their loads in flight: one round trip to
+// memory instead of one a token.
+__device__ __forceinline__ int kv8_grow(unsigned char* codes, int in_block, int need, int old, int lane) {
+    if (in_block == 0) return need;
+    old = min(old, 254);
+    if (need <= old) return old;
+    const float down = kv8_scale(max(127 + old - need, 0));
+    const int bytes = in_block * 128;
+    for (int at = lane * 16; at < bytes; at += 2048) {
+        u32x4 w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) if (at + k * 256 < bytes) w[k] = *(const u32x4*)(codes + at + k * 256);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (at + k * 256 >= bytes) continue;
+            u32x4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const unsigned x = w[k][i]; o[i] = kv8_rescale4(x, down); }
+            *(u32x4*)(codes + at + k * 256) = o;
+        }
+    }
+    return need;
 }
 
 }  // namespace libra
