@@ -121,9 +121,8 @@ struct Kv8ReadArgs {
 // One thread = 8 channels of one row (8 bytes in, 16 out).  e4m3 times a power of two is exact in bf16 (bf16 has the wider exponent
 // and 4 more mantissa bits; below 2^-126 the nearest bf16).
 __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8ReadArgs p) {
-    const int w = blockIdx.z;
-    const long row = blockIdx.x;                      // b * n + i
-    const int b = (int)(row / p.n), t = p.first + (int)(row - (long)b * p.n);
+    const int w = blockIdx.z, b = blockIdx.y, t = p.first + (int)blockIdx.x;
+    const long row = (long)b * p.n + blockIdx.x;
     for (int c = threadIdx.x; c < p.H * 16; c += 256) {
         const int h = c >> 4, sub = c & 15;
         const long head = ((long)w * p.B + b) * p.H + h;
@@ -210,9 +209,9 @@ extern "C" int libra_kv8_read(const uint8_t* codes, const uint8_t* scales, void*
     if (B == 0 || n == 0) return LIBRA_OK;
     const int lg = libra_kv8_geometry_(codes, scales, B, H, capacity, block);
     if (lg < 0) return lg;
-    if (n < 0 || first < 0 || first + n > capacity || ldo < H * 128 || buffer_stride < 0 || B * n > 0x7fffffffL) return LIBRA_ERR_SHAPE;
+    if (n < 0 || first < 0 || first + n > capacity || ldo < H * 128 || buffer_stride < 0 || n > 0xffffffL) return LIBRA_ERR_SHAPE;
     if (!out || !al16(out) || ldo % 8 || buffer_stride % 8) return LIBRA_ERR_ALIGN;
     Kv8ReadArgs a{codes, scales, (bf16_t*)out, (long)ldo, (long)buffer_stride, (int)B, (int)H, lg, (int)capacity, (int)first, (int)n};
-    hipLaunchKernelGGL(kv8_read_kernel, dim3((unsigned)(B * n), 1, 4), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kv8_read_kernel, dim3((unsigned)n, (unsigned)B, 4), dim3(256), 0, (hipStream_t)stream, a);
     return launched();
 }

@@ -6,6 +6,7 @@
 // -inf answers log p = -inf, H = 0.  A row that holds a NaN answers NaN.
 //   dz_v = sum_i g_i ([v = t_i] - p_v) - g_H p_v (log p_v + H),  and 1 - p_v at v = t_i as -expm1(log p_v).
 // HBM-bound: V elements in (forward), V in and V out (backward) a row.
+#include <algorithm>
 #include "hip_common.hpp"
 #include "../../include/libra_hip.h"
 
@@ -84,7 +85,7 @@ __device__ __forceinline__ float lp_wave_sum(float x) {
 }
 
 struct LogprobArgs {
-    const void* z; long ldz; int V; long rows;
+    const void* z; long ldz; int V; long rows, row0;  // this launch's rows begin at row0
     const long long* targets; int T; long long tsub;
     float* logprobs;                                  // [T, rows]
     float* stats;                                     // [3, rows]: max, log1p(r), entropy
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(NT * ROWS, NCH <= 4 && !TOP ? 8 : 4) void logprobs_
     __shared__ float near_one[NEAR];
     __shared__ unsigned long long list[TOP ? LIST : 1];
     __shared__ unsigned nnear, nlist, tau_s, many_s, wtot[NW];
-    const long row = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x >> 6 : 0);
+    const long row = p.row0 + (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x >> 6 : 0);
     if (ROWS > 1 && row >= p.rows) return;
     const T* z = (const T*)p.z + row * p.ldz;
     const int tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
     constexpr int VEC = LpElem<T>::VEC;
     __shared__ float red[4];
     __shared__ unsigned long long redk[4];
-    const long row = blockIdx.x;
+    const long row = p.row0 + blockIdx.x;
     const T* z = (const T*)p.z + row * p.ldz;
     const int nc = (p.V + VEC - 1) / VEC, tid = threadIdx.x;
     auto maxf = [](float a, float b) { return fmaxf(a, b); };
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
 }
 
 struct LogprobBwdArgs {
-    const void* z; long ldz; int V; long rows;
+    const void* z; long ldz; int V; long rows, row0;
     const long long* targets; int T; long long tsub;
     const float* stats; const float* g_lp; const float* g_ent;      // [3, rows]; [T, rows] or null; [rows] or null
     void* dz; long lddz;
@@ -440,7 +441,7 @@ template <typename T, int NT, int ROWS>
 __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBwdArgs p) {
     constexpr int VEC = LpElem<T>::VEC, U = 4;
     constexpr float L2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-    const long row = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / NT : 0);
+    const long row = p.row0 + (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / NT : 0);
     if (ROWS > 1 && row >= p.rows) return;
     const int tid = ROWS > 1 ? threadIdx.x % NT : threadIdx.x;
     const T* z = (const T*)p.z + row * p.ldz;
@@ -530,24 +531,21 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
         dz[v] = LpElem<T>::put(flat ? 0.f : d);
     }
 }
-template <typename T>
-static void lp_launch_bwd(const LogprobBwdArgs& a, hipStream_t st) {
-    if (a.V <= 2048) hipLaunchKernelGGL((logprobs_bwd_kernel<T, 64, 4>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((logprobs_bwd_kernel<T, 256, 1>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
-}
-
 }  // namespace libra
 
 using namespace libra;
+
+constexpr long LP_CHUNK = 1L << 21;                                 // rows of a launch: the threads of a grid are counted in 32 bits
 
 // the smallest workgroup whose registers hold a row
 template <typename T, bool TOP>
 static void lp_launch(const LogprobArgs& a, hipStream_t st) {
     constexpr int W = 8 / LpElem<T>::VEC;                            // pieces are half as wide in fp32
     constexpr int R = TOP ? 1 : 4;                                   // short rows: four waves, four rows a workgroup
-    const dim3 g((unsigned)a.rows);
+    const long rows = std::min(a.rows - a.row0, LP_CHUNK);
+    const dim3 g((unsigned)rows);
     const int P = a.V / LpElem<T>::VEC;                              // whole pieces
-    const dim3 g4((unsigned)((a.rows + R - 1) / R)), t4(64 * R);
+    const dim3 g4((unsigned)((rows + R - 1) / R)), t4(64 * R);
     if (P <= 64 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, W, TOP, R>), g4, t4, 0, st, a);
     else if (P <= 128 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 64, 2 * W, TOP, R>), g4, t4, 0, st, a);
     else if (P <= 1024 * W) hipLaunchKernelGGL((logprobs_row_kernel<T, 256, 4 * W, TOP, 1>), g, dim3(256), 0, st, a);
@@ -556,8 +554,15 @@ static void lp_launch(const LogprobArgs& a, hipStream_t st) {
     else hipLaunchKernelGGL(logprobs_kernel<T>, g, dim3(LP_THREADS), 0, st, a);
 }
 
+template <typename T>
+static void lp_launch_bwd(const LogprobBwdArgs& a, hipStream_t st) {
+    const long rows = std::min(a.rows - a.row0, LP_CHUNK);
+    if (a.V <= 2048) hipLaunchKernelGGL((logprobs_bwd_kernel<T, 64, 4>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((logprobs_bwd_kernel<T, 256, 1>), dim3((unsigned)rows), dim3(256), 0, st, a);
+}
+
 static int lp_check(const void* z, int64_t ldz, int64_t rows, int64_t V, int f32, const int64_t* targets, int64_t n_targets) {
-    if (rows < 0 || rows > 0x7fffffffL || V <= 0 || V > 0x7ffffff0L || ldz < V || n_targets < 0 || n_targets > 64) return LIBRA_ERR_SHAPE;
+    if (rows < 0 || rows > (1L << 40) || V <= 0 || V > 0x7fff0000L || ldz < V || n_targets < 0 || n_targets > 64) return LIBRA_ERR_SHAPE;
     if (!z || ((uintptr_t)z % (f32 ? 4 : 2))) return LIBRA_ERR_ALIGN;
     if (n_targets && !targets) return LIBRA_ERR_ALIGN;
     return LIBRA_OK;
@@ -571,13 +576,16 @@ extern "C" int libra_token_logprobs(const void* logits, int64_t ldz, int64_t row
     if (rc != LIBRA_OK) return rc;
     if (top < 0 || top > 64 || top > V) return LIBRA_ERR_SHAPE;
     if (!stats || (n_targets && !logprobs) || (top && (!top_ids || !top_logprobs))) return LIBRA_ERR_ALIGN;
-    LogprobArgs a{logits, (long)ldz, (int)V, (long)rows, (const long long*)targets, (int)n_targets, (long long)target_sub, logprobs, stats,
+    LogprobArgs a{logits, (long)ldz, (int)V, (long)rows, 0, (const long long*)targets, (int)n_targets, (long long)target_sub, logprobs, stats,
                   (int)top, (long long*)top_ids, top_logprobs};
     const hipStream_t st = (hipStream_t)stream;
-    if (f32) { if (top) lp_launch<float, true>(a, st); else lp_launch<float, false>(a, st); }
-    else if (top) lp_launch<bf16_t, true>(a, st);
-    else lp_launch<bf16_t, false>(a, st);
-    return hipGetLastError() == hipSuccess ? LIBRA_OK : LIBRA_ERR_LAUNCH;
+    for (; a.row0 < a.rows; a.row0 += LP_CHUNK) {
+        if (f32) { if (top) lp_launch<float, true>(a, st); else lp_launch<float, false>(a, st); }
+        else if (top) lp_launch<bf16_t, true>(a, st);
+        else lp_launch<bf16_t, false>(a, st);
+        if (hipGetLastError() != hipSuccess) return LIBRA_ERR_LAUNCH;
+    }
+    return LIBRA_OK;
 }
 
 extern "C" int libra_token_logprobs_bwd(const void* logits, int64_t ldz, int64_t rows, int64_t V, int f32, const int64_t* targets,
@@ -588,9 +596,12 @@ extern "C" int libra_token_logprobs_bwd(const void* logits, int64_t ldz, int64_t
     if (rc != LIBRA_OK) return rc;
     if (lddz < V) return LIBRA_ERR_SHAPE;
     if (!stats || !dlogits || ((uintptr_t)dlogits % (f32 ? 4 : 2)) || (g_logprobs && !targets)) return LIBRA_ERR_ALIGN;
-    LogprobBwdArgs a{logits, (long)ldz, (int)V, (long)rows, (const long long*)targets, (int)n_targets, (long long)target_sub, stats,
+    LogprobBwdArgs a{logits, (long)ldz, (int)V, (long)rows, 0, (const long long*)targets, (int)n_targets, (long long)target_sub, stats,
                      g_logprobs, g_entropy, dlogits, (long)lddz};
-    if (f32) lp_launch_bwd<float>(a, (hipStream_t)stream);
-    else lp_launch_bwd<bf16_t>(a, (hipStream_t)stream);
-    return hipGetLastError() == hipSuccess ? LIBRA_OK : LIBRA_ERR_LAUNCH;
+    for (; a.row0 < a.rows; a.row0 += LP_CHUNK) {
+        if (f32) lp_launch_bwd<float>(a, (hipStream_t)stream);
+        else lp_launch_bwd<bf16_t>(a, (hipStream_t)stream);
+        if (hipGetLastError() != hipSuccess) return LIBRA_ERR_LAUNCH;
+    }
+    return LIBRA_OK;
 }

@@ -1171,7 +1171,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, target_sub: i
     f32 = torch.float32
     lp, stats, tlp = logits.new_empty((T, rows), dtype=f32), logits.new_empty((3, rows), dtype=f32), logits.new_empty((rows, top), dtype=f32)
     ids = targets.new_empty((rows, top))
-    rc = _lib.lib().libra_token_logprobs(logits.data_ptr(), logits.stride(0), rows, V, int(logits.dtype == torch.float32),
+    rc = _lib.lib().libra_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, int(logits.dtype == torch.float32),
                                          targets.data_ptr(), T, target_sub, lp.data_ptr(), stats.data_ptr(), top, ids.data_ptr(),
                                          tlp.data_ptr(), _stream())
     _lib.check(rc, "token_logprobs")
@@ -1194,9 +1194,9 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, stats: torch
     elif out.dtype != logits.dtype or tuple(out.shape) != (rows, V) or out.stride(1) != 1:
         raise ValueError(f"token_logprobs_bwd: out must be row-major {logits.dtype} {(rows, V)}")
     _here("token_logprobs_bwd", stats, g_logprobs, g_entropy, out)
-    rc = _lib.lib().libra_token_logprobs_bwd(logits.data_ptr(), logits.stride(0), rows, V, int(logits.dtype == torch.float32),
+    rc = _lib.lib().libra_token_logprobs_bwd(logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, int(logits.dtype == torch.float32),
                                              targets.data_ptr(), T, target_sub, stats.data_ptr(), _ptr(g_logprobs), _ptr(g_entropy),
-                                             out.data_ptr(), out.stride(0), _stream())
+                                             out.data_ptr(), out.stride(0) if rows > 1 else V, _stream())
     _lib.check(rc, "token_logprobs_bwd")
     return out
 

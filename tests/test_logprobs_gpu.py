@@ -81,7 +81,7 @@ def test_forward(K, rows, V, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("V", [9, 514, 32514])
+@pytest.mark.parametrize("V", [9, 514, 32514, 70003])
 def test_masked_and_forced_rows(K, V, dtype):
     """Columns masked with -inf, with the type's lowest value, rows with one or no column left, forced rows, NaN."""
     z, t = logits(12, V, 3, dtype)
@@ -214,10 +214,35 @@ def test_many_targets_and_empty_calls(K):
     assert K.token_logprobs_bwd(z[:0], t[:, :0].contiguous(), out.stats, None).shape == (0, 50)
 
 
+def test_more_rows_than_a_launch(K):
+    """2^21 rows a launch: the rows behind that limit, an odd number of them."""
+    rows, V = (1 << 21) + 7, 12
+    z = torch.zeros(rows, V, dtype=BF, device="cuda")
+    tail, t2 = logits(9, V, 3, BF)
+    z[-9:] = tail
+    t = torch.zeros((2, rows), dtype=torch.int64, device="cuda")
+    t[:, -9:] = t2
+    out = K.token_logprobs(z, t, top=2)
+    want = check(K, tail, t2, 0, 2)
+    assert torch.equal(out.logprobs[:, -9:], want.logprobs) and torch.equal(out.top_ids[-9:], want.top_ids)
+    assert bool((out.stats[1, :-9] == out.stats[1, 0]).all())
+    g = torch.ones(2, rows, device="cuda")
+    dz = K.token_logprobs_bwd(z, t, out.stats, g)
+    assert torch.equal(dz[-9:], K.token_logprobs_bwd(tail, t2, want.stats, g[:, :9].contiguous())) and torch.equal(dz[0], dz[rows - 10])
+
+
+def test_one_row_of_a_column(K):
+    """A single row whose stride says nothing (as a transposed column has)."""
+    z, t = logits(1, 50, 4, BF)
+    col = z.view(-1).as_strided((1, 50), (1, 1))
+    assert col.stride(0) == 1
+    assert torch.equal(check(K, col, t, 0, 5).logprobs, check(K, z, t, 0, 5).logprobs)
+
+
 def test_refusals(K):
     z, t = logits(3, 50, 1, BF)
     for bad in (lambda: K.token_logprobs(z, t, top=51), lambda: K.token_logprobs(z, t, top=-1), lambda: K.token_logprobs(z.half(), t),
-                lambda: K.token_logprobs(z, t[0]), lambda: K.token_logprobs(z, t.int()), lambda: K.token_logprobs(z.t(), t),
+                lambda: K.token_logprobs(z, t[0]), lambda: K.token_logprobs(z, t.int()), lambda: K.token_logprobs(z.t()[:3], t),
                 lambda: K.token_logprobs(z, t.cpu()), lambda: K.token_logprobs(z, torch.zeros(65, 3, dtype=torch.int64, device="cuda")),
                 lambda: K.token_logprobs_bwd(z, t, torch.zeros(3, 3, dtype=torch.float64, device="cuda"), None),
                 lambda: K.token_logprobs_bwd(z, t, torch.zeros(3, 3, device="cuda"), torch.zeros(1, 3, device="cuda")),

@@ -53,10 +53,30 @@ def test_scores_are_those_of_the_models_logits(name):
     order = R.order(z2, 4)
     assert torch.equal(out.top_ids[:, :, 1:].reshape(-1, 4).cpu(), order)
     near(out.top_logprobs[:, :, 1:].reshape(-1, 4), torch.gather(lp, 1, order), torch.gather(tol, 1, order), "top_logprobs")
-    own = m.token_logprobs(ids, **kw)                   # default labels: the ids where the mask allows
+    # default labels: the ids where the mask allows and the row before can express them
     want = ids.masked_fill(kw["attention_mask"][None] == 0, -100)
+    if name != "unified":
+        vis = kw["vision_indices"] < c["max_vision_token_length"]
+        for b in range(B):
+            for s in range(1, S):
+                for q in range(Q):
+                    if bool(vis[b, s - 1]) != bool(ids[q, b, s] >= c["vocab_size"]):
+                        want[q, b, s] = -100
     with torch.no_grad():
-        assert torch.equal(own.logprobs, m.token_logprobs(ids, want, **kw).logprobs)
+        own = m.token_logprobs(ids, **kw)
+        assert torch.equal(own.logprobs, m.token_logprobs(ids, want, **kw).logprobs) and bool(torch.isfinite(own.logprobs).all())
+
+
+def test_scoring_one_token():
+    """A sequence of a single token: nothing predicts it."""
+    m, _, t, c, _ = _model("default")
+    m.requires_grad_(True)
+    vi = torch.full((1, 1), c["max_vision_token_length"], device="cuda")
+    sig = torch.zeros(1, 1, c["contiguous_signal_size"], dtype=BF, device="cuda")
+    out = m.token_logprobs(torch.full((2, 1, 1), 7, device="cuda"), vision_indices=vi, contiguous_signal=sig, top=2)
+    assert out.logprobs.tolist() == [[[0.0]], [[0.0]]] and out.top_ids.tolist() == [[[[-1, -1]]]] * 2
+    out.logprobs.sum().backward()
+    assert all(p.grad is None or not p.grad.any() for p in m.parameters())
 
 
 @pytest.mark.parametrize("name", ["default", "unified", "pred2d"])
