@@ -439,7 +439,7 @@ struct LogprobBwdArgs {
 // The pieces of a thread that hold a given token (a bit a piece, found first) get that column anew in a rare branch.
 template <typename T, int NT, int ROWS>
 __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBwdArgs p) {
-    constexpr int VEC = LpElem<T>::VEC, U = 4;
+    constexpr int VEC = LpElem<T>::VEC, U = NT > 64 ? 4 : 1;          // pieces whose loads are in flight together (short rows: more waves instead)
     constexpr float L2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
     const long row = p.row0 + (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / NT : 0);
     if (ROWS > 1 && row >= p.rows) return;
