@@ -6,7 +6,7 @@ autograd runs backward on its own thread).
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Sequence
+from typing import Optional, Sequence
 
 import ctypes as C
 import warnings
@@ -1136,13 +1136,27 @@ def bridge_attn_decode8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
 
 
 # ---- log probabilities of given tokens (include/libra_hip.h) ------------------------------------------------------------------
-class TokenLogprobs(NamedTuple):
+class TokenLogprobs:
     """token_logprobs' answer: logprobs fp32 [T, rows]; stats fp32 [3, rows] (row maximum, log of the sum of exp(z - maximum), entropy: what
     the backward takes); top_ids int64 / top_logprobs fp32 [rows, top]."""
-    logprobs: torch.Tensor
-    stats: torch.Tensor
-    top_ids: torch.Tensor
-    top_logprobs: torch.Tensor
+    __slots__ = ("logprobs", "stats", "_top")
+
+    def __init__(self, logprobs: torch.Tensor, stats: torch.Tensor, top=None):
+        self.logprobs, self.stats, self._top = logprobs, stats, top
+
+    def _alternatives(self):
+        if self._top is None:                                          # none were asked for
+            shape = (self.stats.shape[1], 0)
+            self._top = self.stats.new_empty(shape, dtype=torch.int64), self.stats.new_empty(shape)
+        return self._top
+
+    @property
+    def top_ids(self) -> torch.Tensor:
+        return self._alternatives()[0]
+
+    @property
+    def top_logprobs(self) -> torch.Tensor:
+        return self._alternatives()[1]
 
     @property
     def entropy(self) -> torch.Tensor:
@@ -1151,6 +1165,9 @@ class TokenLogprobs(NamedTuple):
     @property
     def lse(self) -> torch.Tensor:
         return self.stats[0] + self.stats[1]
+
+    def __iter__(self):
+        return iter((self.logprobs, self.stats, self.top_ids, self.top_logprobs))
 
 
 def _chk_logprobs(logits, targets, what):
@@ -1169,13 +1186,13 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, target_sub: i
     if top < 0 or top > min(V, 64):
         raise ValueError(f"token_logprobs: top must be 0..{min(V, 64)}, got {top}")
     f32 = torch.float32
-    lp, stats, tlp = logits.new_empty((T, rows), dtype=f32), logits.new_empty((3, rows), dtype=f32), logits.new_empty((rows, top), dtype=f32)
-    ids = targets.new_empty((rows, top))
+    lp, stats = logits.new_empty((T, rows), dtype=f32), logits.new_empty((3, rows), dtype=f32)
+    alt = (targets.new_empty((rows, top)), logits.new_empty((rows, top), dtype=f32)) if top else None
     rc = _lib.lib().libra_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, int(logits.dtype == torch.float32),
-                                         targets.data_ptr(), T, target_sub, lp.data_ptr(), stats.data_ptr(), top, ids.data_ptr(),
-                                         tlp.data_ptr(), _stream())
+                                         targets.data_ptr(), T, target_sub, lp.data_ptr(), stats.data_ptr(), top,
+                                         alt[0].data_ptr() if top else None, alt[1].data_ptr() if top else None, _stream())
     _lib.check(rc, "token_logprobs")
-    return TokenLogprobs(lp, stats, ids, tlp)
+    return TokenLogprobs(lp, stats, alt)
 
 
 def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, g_logprobs: Optional[torch.Tensor],
@@ -1184,11 +1201,13 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, stats: torch
     """dlogits [rows, V] (the logits' type) from the gradients of logprobs [T, rows] and entropy [rows] (fp32, either may be None)."""
     _chk_logprobs(logits, targets, "token_logprobs_bwd")
     (rows, V), T = logits.shape, targets.shape[0]
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (3, rows) or not stats.is_contiguous():
+    f32 = torch.float32
+    if stats.dtype is not f32 or tuple(stats.shape) != (3, rows) or not stats.is_contiguous():
         raise ValueError(f"token_logprobs_bwd: stats must be the forward's fp32 [3, {rows}]")
-    for t, shape, nm in ((g_logprobs, (T, rows), "g_logprobs"), (g_entropy, (rows,), "g_entropy")):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
-            raise ValueError(f"token_logprobs_bwd: {nm} must be contiguous fp32 {shape}")
+    if g_logprobs is not None and (g_logprobs.dtype is not f32 or tuple(g_logprobs.shape) != (T, rows) or not g_logprobs.is_contiguous()):
+        raise ValueError(f"token_logprobs_bwd: g_logprobs must be contiguous fp32 {(T, rows)}")
+    if g_entropy is not None and (g_entropy.dtype is not f32 or tuple(g_entropy.shape) != (rows,) or not g_entropy.is_contiguous()):
+        raise ValueError(f"token_logprobs_bwd: g_entropy must be contiguous fp32 {(rows,)}")
     if out is None:
         out = logits.new_empty((rows, V))
     elif out.dtype != logits.dtype or tuple(out.shape) != (rows, V) or out.stride(1) != 1:
