@@ -168,6 +168,33 @@ def test_mean_negative_logprob_is_the_loss():
         out.backward()
 
 
+def test_two_scorings_in_flight():
+    """Two scoring graphs alive at once (a preferred and a rejected answer): one backward over both == the sum of two, up to the rounding of
+    the bf16 gradients' sum (half a step, 2^-9 relative to the larger of sum and parts); the tokens scored twice agree bit for bit."""
+    import warnings
+    m, _, t, c, _ = _model("default")
+    m.requires_grad_(True)
+    ids, lab, kw = t["in.input_ids"].cuda(), t["in.labels"].cuda(), _inputs(t)
+    other = lab.masked_fill(lab < c["vocab_size"], -100)
+    parts = []
+    for l in (lab, other):
+        m.zero_grad()
+        out = m.token_logprobs(ids, l, **kw)
+        (out.logprobs.sum() / 30 + out.entropy.sum() / 50).backward()
+        parts.append({n: p.grad.float() for n, p in m.named_parameters() if p.grad is not None})
+    m.zero_grad()
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")                 # (the second forward says that it allocates fresh buffers)
+        a, b = m.token_logprobs(ids, lab, **kw), m.token_logprobs(ids, other, **kw)
+    both = other >= 0
+    assert torch.equal(a.logprobs[both], b.logprobs[both])
+    ((a.logprobs.sum() / 30 + a.entropy.sum() / 50) + (b.logprobs.sum() / 30 + b.entropy.sum() / 50)).backward()
+    for n, p in m.named_parameters():
+        if p.grad is not None:
+            x, y = parts[0][n], parts[1][n]
+            assert bool(((p.grad.float() - (x + y)).abs() <= 2.0 ** -8 * torch.maximum((x + y).abs(), torch.maximum(x.abs(), y.abs())) + 1e-30).all()), n
+
+
 def test_scoring_refusals():
     m, _, t, c, _ = _model("default")
     ids, lab, kw = t["in.input_ids"].cuda(), t["in.labels"].cuda(), _inputs(t)
