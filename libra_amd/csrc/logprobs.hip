@@ -361,8 +361,6 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
     }
     m = lp_block(m, maxf, red);
     nan = __syncthreads_or(nan);
-    // which column is the one left out of r: the first that attains m
-    int first = 0x7fffffff;
     float s = 0.f, t = 0.f;
     for (int c = tid; c < nc; c += LP_THREADS) {
         float f[VEC];
@@ -372,13 +370,12 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LogprobArgs 
             const int v = c * VEC + e;
             if (v >= p.V) continue;
             const float d = lp_diff(f[e], m);
-            if (d == 0.f) { if (v < first) first = v; }
             const float ex = __expf(d);
             s += d == 0.f ? 0.f : ex;
             t += ex > 0.f ? ex * d : 0.f;
         }
     }
-    int equal = 0;                                     // columns that attain m beyond the first
+    int equal = 0;                                     // columns that attain m: all but one of them belong to r
     for (int c = tid; c < nc; c += LP_THREADS) {
         float f[VEC];
         lp_load(z, p.V, c, f);
