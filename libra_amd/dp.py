@@ -72,6 +72,36 @@ def _is_nccl(group) -> bool:
     return dist.is_initialized() and dist.get_backend(group) == "nccl"
 
 
+def _staged(t: torch.Tensor, group) -> bool:
+    return t.is_cuda and not _is_nccl(group)
+
+
+class _StagedWork:
+    """A collective on host copies; wait() brings the result back, once."""
+
+    def __init__(self, work, host: torch.Tensor, dst: torch.Tensor):
+        self.work, self.host, self.dst = work, host, dst
+
+    def wait(self):
+        if self.work is not None:
+            self.work.wait()
+            self.dst.copy_(self.host)
+            self.work = self.host = None
+
+
+def _collective(fn: Callable, out: torch.Tensor, inp: Optional[torch.Tensor] = None, *, group=None, **kw):
+    """fn(out[, inp], async_op=True) on RCCL or on host tensors as it stands.  gloo gets host tensors only: its collectives on device
+    tensors copy from threads and streams of their own, which has hung where ranks share a GPU; device tensors of a gloo group are
+    copied to host memory first (synchronously, behind the current stream's work) and back by wait()."""
+    if not _staged(out, group):
+        return fn(*((out,) if inp is None else (out, inp)), group=group, async_op=True, **kw)
+    if inp is None:
+        host = out.to("cpu", copy=True)
+        return _StagedWork(fn(host, group=group, async_op=True, **kw), host, out)
+    host = torch.empty(out.shape, dtype=out.dtype)
+    return _StagedWork(fn(host, inp.to("cpu", copy=True), group=group, async_op=True, **kw), host, out)
+
+
 class _Bucket:
     __slots__ = ("flat", "names", "slots", "ready", "work", "launched", "shard")
 
@@ -212,17 +242,17 @@ class GradBuckets:
         nb = b.flat.numel() * b.flat.element_size()
         if self.mode == "allreduce":
             op = dist.ReduceOp.AVG if _is_nccl(self.group) else dist.ReduceOp.SUM
-            b.work = [dist.all_reduce(b.flat, op=op, group=self.group, async_op=True)]
+            b.work = [_collective(dist.all_reduce, b.flat, op=op, group=self.group)]
             self.bytes_exchanged += 2 * nb * (self.world - 1) // self.world
         else:
             lo, hi = b.shard
             op = dist.ReduceOp.AVG if _is_nccl(self.group) else dist.ReduceOp.SUM
-            b.work = [dist.reduce_scatter_tensor(b.flat[lo:hi], b.flat, op=op, group=self.group, async_op=True)]
+            b.work = [_collective(dist.reduce_scatter_tensor, b.flat[lo:hi], b.flat, op=op, group=self.group)]
             self.bytes_exchanged += nb * (self.world - 1) // self.world
             if self.mode == "rs_ag":
                 if not _is_nccl(self.group):          # RCCL runs a group's collectives in issue order on its stream; gloo's
                     b.work[0].wait()                  # worker threads do not - keep the pair ordered there (CPU tests only)
-                b.work.append(dist.all_gather_into_tensor(b.flat, b.flat[lo:hi], group=self.group, async_op=True))
+                b.work.append(_collective(dist.all_gather_into_tensor, b.flat, b.flat[lo:hi], group=self.group))
                 self.bytes_exchanged += nb * (self.world - 1) // self.world
 
     def wait_bucket(self, b: _Bucket):
@@ -295,7 +325,7 @@ class GradBuckets:
             lo, hi = b.shard if sharded else (0, b.flat.numel())
             sumsq_fn(b.flat[lo:hi], out, accumulate=i > 0)
         if sharded:
-            dist.all_reduce(out, op=dist.ReduceOp.SUM, group=self.group)
+            _collective(dist.all_reduce, out, op=dist.ReduceOp.SUM, group=self.group).wait()
         return out
 
 
@@ -397,7 +427,7 @@ class FlatAdamW:
                 self.update_fn(st["master"][s:e], st["m"][s:e], st["v"][s:e], b.flat[lo + s:lo + e], pf[lo + s:lo + e],
                                lr=lr, beta1=b1, beta2=b2, eps=self.eps, weight_decay=wd, bias_corr1=bc1, bias_corr2=bc2, **clip)
             if self.shard:
-                works.append(dist.all_gather_into_tensor(pf, pf[lo:st["hi"]], group=self.buckets.group, async_op=True))
+                works.append(_collective(dist.all_gather_into_tensor, pf, pf[lo:st["hi"]], group=self.buckets.group))
         for w in works:
             w.wait()
 
@@ -472,4 +502,4 @@ class FlatAdamW:
         self.t = int(sd["t"])
         if self.shard:
             for pf, st in zip(self.pflat, self.state):
-                dist.all_gather_into_tensor(pf, pf[st["lo"]:st["hi"]], group=self.buckets.group)
+                _collective(dist.all_gather_into_tensor, pf, pf[st["lo"]:st["hi"]], group=self.buckets.group).wait()

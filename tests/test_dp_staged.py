@@ -1,0 +1,84 @@
+"""Device tensors of a gloo group go through host memory (dp._collective): the same workers as on host tensors, with the staging forced on
+host tensors - every result equals the unstaged one bit for bit, and no collective is handed a tensor the caller holds."""
+import numpy as np
+import pytest
+import torch
+import torch.distributed as dist
+
+import test_dp_gloo as G
+
+
+def _staged(rank, world, port, q, worker, *args):
+    from libra_amd import dp
+    dp._staged = lambda t, group: True
+    held, seen = set(), []
+    for name in ("all_reduce", "reduce_scatter_tensor", "all_gather_into_tensor"):
+        def wrapped(*ts, _fn=getattr(dist, name), **kw):
+            seen.extend(t.untyped_storage().data_ptr() for t in ts)
+            return _fn(*ts, **kw)
+        setattr(dist, name, wrapped)
+    init = dp.GradBuckets.__init__
+
+    def hold(self, *a, **kw):
+        init(self, *a, **kw)
+        held.update(b.flat.untyped_storage().data_ptr() for b in self.buckets)
+    dp.GradBuckets.__init__ = hold
+    worker(rank, world, port, q, *args)
+    assert seen and held and not held & set(seen)
+
+
+def _run(worker, *args):
+    ctx = G.mp.get_context("spawn")
+    q, port = ctx.Queue(), G._free_port()
+    ps = [ctx.Process(target=_staged, args=(r, 2, port, q, worker, *args)) for r in range(2)]
+    [p.start() for p in ps]
+    res = sorted((q.get(timeout=180) for _ in range(2)), key=lambda t: t[0])
+    [p.join(60) for p in ps]
+    assert all(p.exitcode == 0 for p in ps)
+    return res
+
+
+def _same(a, b):
+    if isinstance(a, dict):
+        assert a.keys() == b.keys()
+        for k in a:
+            _same(a[k], b[k])
+    elif isinstance(a, (list, tuple)):
+        assert len(a) == len(b)
+        for x, y in zip(a, b):
+            _same(x, y)
+    elif isinstance(a, np.ndarray):
+        assert np.array_equal(a, b)
+    else:
+        assert a == b
+
+
+@pytest.mark.parametrize("mode", ["allreduce", "rs_ag"])
+def test_staged_exchange(mode):
+    _same(_run(G._worker_modes, mode), G._run(G._worker_modes, 2, mode))
+
+
+@pytest.mark.parametrize("mode", ["allreduce", "zero1"])
+def test_staged_sharded_optimizer(mode):
+    _same(_run(G._worker_zero1, mode), G._run(G._worker_zero1, 2, mode))
+
+
+@pytest.mark.parametrize("mode", ["allreduce", "zero1"])
+def test_staged_clipping_and_resume(mode):
+    _same(_run(G._worker_clip, mode), G._run(G._worker_clip, 2, mode))
+
+
+def test_wait_copies_once():
+    from libra_amd import dp
+
+    class Work:
+        n = 0
+
+        def wait(self):
+            Work.n += 1
+    dst, host = torch.zeros(3), torch.ones(3)
+    w = dp._StagedWork(Work(), host, dst)
+    w.wait()
+    dst.add_(1)
+    w.wait()
+    assert Work.n == 1 and dst.tolist() == [2, 2, 2]
