@@ -339,9 +339,11 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
     def token_logprobs(self, input_ids: torch.LongTensor, labels: Optional[torch.LongTensor] = None, *,
                        attention_mask: Optional[torch.Tensor] = None, vision_indices: Optional[torch.LongTensor] = None,
                        contiguous_signal: Optional[torch.Tensor] = None, top: int = 0) -> LibraTokenLogprobs:
-        """Score given tokens: log probability of labels [Q, B, S] (< 0: not scored; default: the input ids, where attention_mask allows
-        and the row before has the token in its head - with routed heads a text row never predicts an image id nor the reverse: the
-        switches between modalities are forced, not predicted) under the uncached forward, with each predicting distribution's entropy and its `top` (<= 64) most likely ids.
+        """Score given tokens: log probability of labels [Q, B, S] (< 0: not scored) under the uncached forward, with each predicting
+        distribution's entropy and its `top` (<= 64) most likely ids.  Default labels: the input ids, where attention_mask allows both the
+        token and the row before, which predicts it (the first token behind left padding is predicted by nothing, like position 0), and
+        that row has the token in its head - with routed heads a text row never predicts an image id nor the reverse: the switches between
+        modalities are forced, not predicted.  Labels that are given are scored as they stand.
         logprobs and entropy carry a gradient to the parameters - the losses that `labels=` of forward() does not cover (a reward- or
         preference-weighted log likelihood, an entropy bonus) are ordinary expressions of them."""
         if vision_indices is None:
@@ -357,7 +359,8 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
         if attention_mask is None:
             attention_mask = torch.ones((B, S), dtype=torch.bool, device=input_ids.device)
         if labels is None:
-            labels = input_ids.masked_fill(attention_mask[None] == 0, -100)
+            row_before = torch.nn.functional.pad(attention_mask[:, :-1] != 0, (1, 0), value=True)
+            labels = input_ids.masked_fill(((attention_mask == 0) | ~row_before)[None], -100)
             if not self._dims.unified_head:
                 row_is_vision = torch.nn.functional.pad(vision_indices[:, :-1] < self.max_vision_token_length, (1, 0))
                 labels = labels.masked_fill(row_is_vision[None] != (input_ids >= self.config.vocab_size), -100)

@@ -1,0 +1,59 @@
+"""LibraForCausalLM.token_logprobs without a GPU: which positions its default labels score, with the autograd node replaced by a recorder
+(host tensors that call themselves device tensors)."""
+import pytest
+import torch
+
+from helpers import load_golden
+from libra_amd.libra import LibraConfig, LibraForCausalLM
+from libra_amd.libra import modeling_libra as M
+
+
+class Device(torch.Tensor):
+    """A host tensor that passes the entry point's device check."""
+    is_cuda = True
+
+
+def _default_labels(monkeypatch, unified, mask, vision_indices, ids):
+    _, meta = load_golden("libra_tiny.safetensors")
+    m = LibraForCausalLM(LibraConfig(**dict(meta["cfg"], unified_head=unified)))
+    seen = {}
+
+    def record(model, holder, names, input_ids, attention_mask, vision_indices, signal, labels, top, *params):
+        seen["labels"] = labels
+        holder.update(top_ids=None, top_logprobs=None)
+        return None, None
+    monkeypatch.setattr(M._LibraScoreFunction, "apply", staticmethod(record))
+    m.token_logprobs(ids.as_subclass(Device), attention_mask=mask, vision_indices=vision_indices)
+    return seen["labels"].as_subclass(torch.Tensor), m
+
+
+@pytest.mark.parametrize("unified", [False, True])
+@pytest.mark.parametrize("kind", [torch.bool, torch.int64])
+def test_default_labels_leave_out_what_a_padding_row_would_predict(monkeypatch, unified, kind):
+    """Row t - 1 predicts token t: the first token behind left padding is predicted by nothing, like the token at position 0."""
+    _, meta = load_golden("libra_tiny.safetensors")
+    L, S = meta["cfg"]["max_vision_token_length"], 6
+    mask = torch.tensor([[0, 0, 1, 1, 1, 1], [1, 1, 1, 1, 1, 1], [1, 1, 1, 0, 0, 0], [0, 0, 0, 0, 0, 1]]).to(kind)
+    ids = torch.arange(5, 5 + 4 * S).view(1, 4, S).repeat(2, 1, 1)
+    labels, _ = _default_labels(monkeypatch, unified, mask, torch.full((4, S), L), ids)
+    scored = labels >= 0
+    first = [2, 0, 0, 5]
+    for b in range(4):
+        for s in range(S):
+            # (position 0 has a label with either head, and scoring answers 0 there: nothing predicts it)
+            want = s == 0 if s == first[b] else bool(mask[b, s])
+            assert scored[:, b, s].tolist() == [want] * 2, (b, s)
+    assert torch.equal(labels[scored], ids[scored])
+
+
+@pytest.mark.parametrize("pad", [1, 3])
+def test_default_labels_do_not_depend_on_the_padding(monkeypatch, pad):
+    """An image and text, alone and left-padded: the same tokens are scored."""
+    _, meta = load_golden("libra_tiny.safetensors")
+    L, V = meta["cfg"]["max_vision_token_length"], meta["cfg"]["vocab_size"]
+    ids = torch.tensor([3, V + 1, V + 2, V + 4, 9, 8])[None, None].repeat(2, 1, 1)
+    vi = torch.tensor([[L, 0, 1, L - 1, L, L]])
+    alone, _ = _default_labels(monkeypatch, False, torch.ones(1, 6, dtype=torch.bool), vi, ids)
+    wide = lambda x, v: torch.nn.functional.pad(x, (pad, 0), value=v)  # noqa: E731
+    padded, _ = _default_labels(monkeypatch, False, wide(torch.ones(1, 6), 0) > 0, wide(vi, L), wide(ids, 0))
+    assert torch.equal(padded[:, :, pad + 1:], alone[:, :, 1:]) and bool((padded[:, :, :pad + 1] < 0).all())

@@ -353,3 +353,24 @@ def test_fp8_cache_with_variants(name):
         res.append(torch.cat(z, 2))
     fin = torch.isfinite(res[0])
     assert torch.equal(fin, torch.isfinite(res[1])) and rel_err(res[1][fin], res[0][fin]) < 0.2
+
+
+def test_default_scores_do_not_depend_on_left_padding():
+    """Row 0 of the generation fixture is left-padded by 4: the same tokens are scored as with the prompt alone, with the same values.  The two
+    runs' logits agree within 1e-2 of their largest (the bound that the padded prompt's own test holds them to: other key tiles, bf16);
+    log p = z_t - lse, and the entropy, a mean of such differences, move by at most twice that each (entropy: by its probabilities as well,
+    which move by twice the logits' error relative, times the spread of log p, log V + the range of the logits)."""
+    m, t, meta = _gen()
+    ids, vi, sig, am = (t[f"in.{k}"].cuda() for k in ("input_ids", "vision_indices", "signal", "attention_mask"))
+    sig = sig.to(BF)
+    assert am[0].tolist()[:5] == [0, 0, 0, 0, 1]
+    with torch.no_grad():
+        z = m(input_ids=ids[:, :1, 4:], vision_indices=vi[:1, 4:], contiguous_signal=sig[:1, 4:]).logits.float()
+        wide = m.token_logprobs(ids, attention_mask=am, vision_indices=vi, contiguous_signal=sig)
+        alone = m.token_logprobs(ids[:, :1, 4:], vision_indices=vi[:1, 4:], contiguous_signal=sig[:1, 4:])
+    d = 1e-2 * float(z[torch.isfinite(z)].abs().max())
+    spread = float(torch.log(torch.tensor(float(z.shape[-1])))) + 2 * float(z[torch.isfinite(z)].abs().max())
+    assert not wide.logprobs[:, 0, :5].any() and not wide.entropy[:, 0, :5].any()
+    assert torch.equal(wide.logprobs[:, 0, 4:] != 0, alone.logprobs[:, 0] != 0) and int((alone.logprobs != 0).sum()) > 0
+    assert float((wide.logprobs[:, 0, 4:] - alone.logprobs[:, 0]).abs().max()) <= 2 * d
+    assert float((wide.entropy[:, 0, 4:] - alone.entropy[:, 0]).abs().max()) <= 2 * d + 2 * d * spread
