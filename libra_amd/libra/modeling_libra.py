@@ -549,11 +549,14 @@ class _LibraScoreFunction(torch.autograd.Function):
         need = holder["grad_on"] and any(ctx.needs_input_grad[9:])
         out = DE.forward(sd, packed, model._dims, input_ids, attention_mask, vision_indices, signal, labels, save=need,
                          recompute=need and model.model.gradient_checkpointing and model.training, score=top)
-        sc = out["scores"]
-        holder["top_ids"], holder["top_logprobs"] = sc["top_ids"], sc["top_logprobs"]
-        ctx.model, ctx.sd, ctx.out, ctx.names = model, sd, out, names
+        # nothing that ctx keeps may lead to a returned tensor: the node belongs to both outputs, and Python's collector does not see
+        # through a cycle with two owners outside it - every call's activations would stay for good
+        answer = {k: out["scores"].pop(k) for k in ("logprobs", "entropy", "top_ids", "top_logprobs")}
+        holder["top_ids"], holder["top_logprobs"] = answer["top_ids"], answer["top_logprobs"]
+        ctx.model, ctx.sd, ctx.names = model, sd, names
+        ctx.out = out if need else {}
         ctx.want = {n for n, ng in zip(names, ctx.needs_input_grad[9:]) if ng}
-        return sc["logprobs"], sc["entropy"]
+        return answer["logprobs"], answer["entropy"]
 
     @staticmethod
     def backward(ctx, g_lp, g_ent):
@@ -565,7 +568,7 @@ class _LibraScoreFunction(torch.autograd.Function):
         for n in ctx.names:
             gr = grads.get(n) if n in ctx.want and not dp.is_captured(n) else None      # captured: lives in the DP bucket
             res.append(gr.reshape(ctx.sd[n].shape) if gr is not None else None)
-        ctx.out["saved"] = None
+        ctx.out = {}                                        # (the logits too: an output that is kept must not keep them)
         return (None,) * 9 + tuple(res)
 
 

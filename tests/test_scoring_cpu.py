@@ -1,5 +1,9 @@
 """LibraForCausalLM.token_logprobs without a GPU: which positions its default labels score, with the autograd node replaced by a recorder
 (host tensors that call themselves device tensors)."""
+import gc
+import types
+import weakref
+
 import pytest
 import torch
 
@@ -57,3 +61,60 @@ def test_default_labels_do_not_depend_on_the_padding(monkeypatch, pad):
     wide = lambda x, v: torch.nn.functional.pad(x, (pad, 0), value=v)  # noqa: E731
     padded, _ = _default_labels(monkeypatch, False, wide(torch.ones(1, 6), 0) > 0, wide(vi, L), wide(ids, 0))
     assert torch.equal(padded[:, :, pad + 1:], alone[:, :, 1:]) and bool((padded[:, :, :pad + 1] < 0).all())
+
+
+class _State:
+    pass
+
+
+class _Engine:
+    """Stands in for the decoder engine: a forward whose saved state is one object that can be watched."""
+
+    def __init__(self, monkeypatch):
+        self.alive = []
+        monkeypatch.setattr(M.DE, "forward", self.forward)
+        monkeypatch.setattr(M.DE, "backward", lambda sd, packed, dims, out, want, g_scores: {
+            n: g_scores[0].sum() + 2 * g_scores[1].sum() + torch.zeros(3) for n in want if out["saved"]["x"]})
+        self.model = types.SimpleNamespace(_refresh_packed=lambda sd: None, _dims=None, _packed=None, training=True,
+                                           model=types.SimpleNamespace(gradient_checkpointing=False))
+
+    def forward(self, sd, packed, dims, ids, mask, vi, signal, labels, *, save, recompute, score):
+        state = _State()
+        self.alive.append(weakref.ref(state))
+        scores = dict(logprobs=torch.zeros(2, 1, 4), entropy=torch.zeros(2, 1, 4), top_ids=torch.zeros(2, 1, 4, 0), top_logprobs=torch.zeros(2, 1, 4, 0),
+                      parts=[state], scored=torch.ones(2, 4))
+        return dict(scores=scores, z_lang=state, saved=dict(scores=scores, x=[state]) if save else None)
+
+    def call(self, p, grad_on=True):
+        return M._LibraScoreFunction.apply(self.model, dict(grad_on=grad_on), ["w"], None, None, None, None, None, 0, p)
+
+
+@pytest.mark.parametrize("mode", ["both", "logprobs", "entropy", "dropped", "not saved"])
+def test_a_scoring_call_is_freed_with_its_outputs(monkeypatch, mode):
+    """Nothing of a call outlives its outputs, without the collector's help: activations (and with them the row arena's lease) go at once."""
+    e = _Engine(monkeypatch)
+    p = torch.nn.Parameter(torch.zeros(3))
+    gc.disable()
+    try:
+        for _ in range(3):
+            lp, ent = e.call(p, mode != "not saved")
+            if mode == "both":
+                (lp.sum() + ent.sum()).backward()
+            elif mode in ("logprobs", "entropy"):
+                (lp if mode == "logprobs" else ent).sum().backward()
+            del lp, ent
+            assert [r() for r in e.alive] == [None] * len(e.alive)
+    finally:
+        gc.enable()
+    assert (p.grad is None) == (mode in ("dropped", "not saved"))
+
+
+def test_a_backward_frees_the_call_and_is_the_only_one(monkeypatch):
+    e = _Engine(monkeypatch)
+    p = torch.nn.Parameter(torch.zeros(3))
+    lp, ent = e.call(p)
+    both = lp.sum() + ent.sum()
+    both.backward(retain_graph=True)
+    assert e.alive[0]() is None and p.grad.tolist() == [24.0] * 3          # (lp and ent are still held)
+    with pytest.raises(RuntimeError, match="ran already"):
+        both.backward()

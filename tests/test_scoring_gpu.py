@@ -374,3 +374,26 @@ def test_default_scores_do_not_depend_on_left_padding():
     assert torch.equal(wide.logprobs[:, 0, 4:] != 0, alone.logprobs[:, 0] != 0) and int((alone.logprobs != 0).sum()) > 0
     assert float((wide.logprobs[:, 0, 4:] - alone.logprobs[:, 0]).abs().max()) <= 2 * d
     assert float((wide.entropy[:, 0, 4:] - alone.entropy[:, 0]).abs().max()) <= 2 * d + 2 * d * spread
+
+
+def test_scoring_leaves_nothing_behind():
+    """Call after call - backward over both outputs, over one, or none - the memory in use stays where it was, and the row arena is free again."""
+    import gc
+    m, _, t, c, _ = _model("default")
+    m.requires_grad_(True)
+    ids, lab, kw = t["in.input_ids"].cuda(), t["in.labels"].cuda(), _inputs(t)
+    gc.collect()                                        # (what earlier tests left in cycles)
+    gc.disable()
+    try:
+        used = []
+        for i in range(7):
+            out = m.token_logprobs(ids, lab, top=2, **kw)
+            if i % 3 < 2:
+                (out.logprobs.sum() + (out.entropy.sum() if i % 3 == 0 else 0)).backward()
+            del out
+            m.zero_grad()
+            assert m._packed.arena is None or not m._packed.arena.busy, i
+            used.append(torch.cuda.memory_allocated())
+        assert len(set(used[3:])) == 1, used            # (the first three bring the operands and the arena's buffers)
+    finally:
+        gc.enable()
