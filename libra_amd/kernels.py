@@ -910,8 +910,29 @@ def rmsnorm_routed(x, w_lang, w_vis, flag, eps: float, *, out=None, save_rstd: b
     return (y, rstd) if save_rstd else y
 
 
-def rope_bridge(qkv, tb, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, S: int, H: int):
+def _chk_rope(what: str, qkv, tb, weights, flag, cos, sin, H: int) -> None:
+    """The operands of a rope_bridge launch, which reads N = len(qkv) rows of 3 H 128 and 16 columns, N flags, four [H 128, 8] matrices and
+    two tables of 128 columns: every one of them as large as that and on qkv's device."""
     _chk2d(qkv, "qkv"); _chk2d(tb, "tb")
+    N, W = qkv.shape[0], H * 128
+    if qkv.shape[1] < 3 * W or tb.shape[0] < N or tb.shape[1] < 16:
+        raise ValueError(f"{what}: qkv must be [N, {3 * W}] and tb [N, >= 16], got {tuple(qkv.shape)} and {tuple(tb.shape)}")
+    if flag.dtype is not torch.uint8 or flag.numel() < N or not flag.is_contiguous():
+        raise ValueError(f"{what}: flag must be contiguous uint8 [{N}], got {flag.dtype} {tuple(flag.shape)}")
+    for w in weights:
+        if w.dtype is not BF16 or tuple(w.shape) != (W, 8) or not w.is_contiguous():
+            raise ValueError(f"{what}: the bridge weights are contiguous bf16 [{W}, 8], got {w.dtype} {tuple(w.shape)} strides {w.stride()}")
+    for t in (cos, sin):
+        if t.dtype is not BF16 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != 128 or not t.is_contiguous():
+            raise ValueError(f"{what}: cos and sin are contiguous bf16 [positions, 128], got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
+    at = qkv.get_device()
+    for t in (tb, flag, cos, sin, *weights):
+        if t.get_device() != at:
+            raise ValueError(f"{what}: every tensor must be on qkv's device, {qkv.device}, got {t.device}")
+
+
+def rope_bridge(qkv, tb, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, S: int, H: int):
+    _chk_rope("rope_bridge", qkv, tb, (bk_l, bk_v, bv_l, bv_v), flag, cos, sin, H)
     N = qkv.shape[0]
     kc = torch.empty((N, H * 128), dtype=BF16, device=qkv.device)
     vc = torch.empty((N, H * 128), dtype=BF16, device=qkv.device)
@@ -927,10 +948,10 @@ def rope_bridge_pos(qkv, tb, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, positions, 
     """rope_bridge with explicit int32 positions: [N] (cached decode step, left-padded prompts) or [N, 2] (use_2d_rope: even heads
     rotate by column 0, odd heads by column 1).  `append` = (caches, slot): a generation step (row n = sequence n) - the four K / V
     rows of every new token are also stored at `slot` (cuda int64 [1]) of the layer's four caches [B, Lmax, H*128] in this launch."""
-    _chk2d(qkv, "qkv"); _chk2d(tb, "tb")
+    _chk_rope("rope_bridge_pos", qkv, tb, (bk_l, bk_v, bv_l, bv_v), flag, cos, sin, H)
     N = qkv.shape[0]
-    if positions.dtype != torch.int32 or positions.numel() not in (N, 2 * N) or not positions.is_contiguous():
-        raise ValueError("rope_bridge_pos: positions must be contiguous int32 [N] or [N, 2]")
+    if positions.dtype != torch.int32 or positions.numel() not in (N, 2 * N) or not positions.is_contiguous() or positions.device != qkv.device:
+        raise ValueError("rope_bridge_pos: positions must be contiguous int32 [N] or [N, 2] on qkv's device")
     pstride = positions.numel() // N
     kc = torch.empty((N, H * 128), dtype=BF16, device=qkv.device)
     vc = torch.empty((N, H * 128), dtype=BF16, device=qkv.device)
@@ -1076,7 +1097,7 @@ def rope_bridge_pos_append8(qkv, tb, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, pos
     """A generation step's rope_bridge_pos with an 8-bit cache: q and K_same rotated in place, the four rows of every new token (row n =
     sequence n) quantised into slot `slot` (cuda int64 [1]) in the same launch - rope_bridge_pos followed by kv8_append, bit for bit."""
     B, Hc, cap, block = _kv8_geometry(codes, scales, "rope_bridge_pos_append8")
-    _chk2d(qkv, "qkv"); _chk2d(tb, "tb")
+    _chk_rope("rope_bridge_pos_append8", qkv, tb, (bk_l, bk_v, bv_l, bv_v), flag, cos, sin, H)
     if qkv.shape[0] != B or tb.shape[0] != B or Hc != H or qkv.shape[1] != 3 * H * 128:
         raise ValueError(f"rope_bridge_pos_append8: qkv must be [{B}, {3 * Hc * 128}] for this cache, got {tuple(qkv.shape)}")
     if positions.dtype != torch.int32 or positions.numel() not in (B, 2 * B) or not positions.is_contiguous():

@@ -135,3 +135,65 @@ def test_host_wrappers_refuse_without_a_gpu():
         K.kv8_append(rows, codes, scales, torch.zeros(1, dtype=torch.int64))                        # host tensors
     with pytest.raises(ValueError):
         K.kv8_append(rows[:3], codes, scales, torch.zeros(1, dtype=torch.int64))
+
+
+# ---- operands of the rotary + bridge launches: tensors of a device that is not there, a library that only records --------------------
+ROPE = ("rope_bridge", "rope_bridge_pos", "rope_bridge_pos_append8")
+
+
+def _rope_call(monkeypatch, name, N=2, H=2, **change):
+    """The entry point on fake device tensors -> the name of the library call it made."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from libra_amd import kernels as K
+    made = []
+
+    class Library:
+        def __getattr__(self, fn):
+            return lambda *a: made.append(fn) or 0
+    monkeypatch.setattr(K._lib, "lib", Library)
+    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    bf, D = torch.bfloat16, H * 128
+    with FakeTensorMode():
+        e = lambda *s, dtype=bf, device="cuda": torch.empty(*s, dtype=dtype, device=device)  # noqa: E731
+        a = dict(qkv=e(N, 3 * D), tb=e(N, 64), bk_l=e(D, 8), bk_v=e(D, 8), bv_l=e(D, 8), bv_v=e(D, 8), flag=e(N, dtype=torch.uint8),
+                 cos=e(64, 128), sin=e(64, 128))
+        a.update({k: v(e) for k, v in change.items() if k in a})
+        if name == "rope_bridge":
+            K.rope_bridge(*a.values(), 1, H)
+        else:
+            pos = change.get("positions", lambda e: e(N, dtype=torch.int32))(e)
+            if name == "rope_bridge_pos":
+                K.rope_bridge_pos(*a.values(), pos, H)
+            else:
+                K.rope_bridge_pos_append8(*a.values(), pos, H, e(4, N, H, 32, 128, dtype=torch.uint8), e(4, N, H, 2, dtype=torch.uint8),
+                                          e(1, dtype=torch.int64))
+    return made[-1]
+
+
+@pytest.mark.parametrize("name", ROPE)
+def test_rope_operands_are_taken(monkeypatch, name):
+    assert _rope_call(monkeypatch, name) == "libra_" + name
+    assert _rope_call(monkeypatch, name, qkv=lambda e: e(2, 3 * 256 + 64)[:, :768], tb=lambda e: e(2, 3 * 256 + 64)[:, 768:]) == "libra_" + name
+
+
+@pytest.mark.parametrize("name", ROPE)
+@pytest.mark.parametrize("what,bad", [
+    ("flag", lambda e: e(1, dtype=torch.uint8)), ("flag", lambda e: e(2, dtype=torch.int64)), ("flag", lambda e: e(4, dtype=torch.uint8)[::2]),
+    ("flag", lambda e: e(2, dtype=torch.uint8, device="cpu")),
+    ("tb", lambda e: e(2, 8)), ("tb", lambda e: e(1, 64)),
+    ("bk_l", lambda e: e(128, 8)), ("bk_v", lambda e: e(256, 4)), ("bv_l", lambda e: e(256, 8, dtype=torch.float32)), ("bv_v", lambda e: e(8, 256).t()),
+    ("bk_l", lambda e: e(256, 8, device="cpu")),
+    ("cos", lambda e: e(64, 64)), ("sin", lambda e: e(32, 128)), ("cos", lambda e: e(64, 128, dtype=torch.float32)), ("sin", lambda e: e(64, 128, device="cpu")),
+    ("sin", lambda e: e(64, 256)[:, :128]), ("qkv", lambda e: e(2, 1024)[:, :640])])
+def test_rope_operands_are_refused(monkeypatch, name, what, bad):
+    """What the launch would read outside of: too few flags, weights or table rows, another type, another device."""
+    with pytest.raises(ValueError):
+        _rope_call(monkeypatch, name, **{what: bad})
+
+
+@pytest.mark.parametrize("name", ROPE[1:])
+@pytest.mark.parametrize("bad", [lambda e: e(1, dtype=torch.int32), lambda e: e(2, dtype=torch.int64), lambda e: e(2, dtype=torch.int32, device="cpu")])
+def test_rope_positions_are_refused(monkeypatch, name, bad):
+    with pytest.raises(ValueError):
+        _rope_call(monkeypatch, name, positions=bad)
