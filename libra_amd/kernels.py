@@ -1065,7 +1065,7 @@ def _kv8_rows(rows, n: int, width: int, what: str):
         if r.dtype is not BF16 or tuple(r.shape) != (n, width) or st[1] != 1:
             raise ValueError(f"{what}: rows must be row-major bf16 [{n}, {width}], got {r.dtype} {tuple(r.shape)} strides {st}")
         args.append(r.data_ptr())
-        args.append(st[0])
+        args.append(st[0] if n > 1 else width)                       # (one row: its stride says nothing)
     return args
 
 
@@ -1107,7 +1107,8 @@ def rope_bridge_pos_append8(qkv, tb, bk_l, bk_v, bv_l, bv_v, flag, cos, sin, pos
     if B == 0:
         return
     _here("rope_bridge_pos_append8", qkv, tb, flag, positions, codes, scales, slot)
-    rc = _lib.lib().libra_rope_bridge_pos_append8(qkv.data_ptr(), qkv.stride(0), tb.data_ptr(), tb.stride(0), bk_l.data_ptr(),
+    ld, ldt = (qkv.stride(0), tb.stride(0)) if B > 1 else (3 * H * 128, 16)          # (one row: its stride says nothing)
+    rc = _lib.lib().libra_rope_bridge_pos_append8(qkv.data_ptr(), ld, tb.data_ptr(), ldt, bk_l.data_ptr(),
                                                   bk_v.data_ptr(), bv_l.data_ptr(), bv_v.data_ptr(), flag.data_ptr(), cos.data_ptr(),
                                                   sin.data_ptr(), cos.shape[0], B, positions.data_ptr(), positions.numel() // B, H,
                                                   codes.data_ptr(), scales.data_ptr(), cap, block, slot.data_ptr(), _stream())
@@ -1148,8 +1149,8 @@ def bridge_attn_decode8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     out = q.new_empty((B, H * 128))
     nbytes = _lib.lib().libra_bridge_attn_decode8_workspace_bytes(B, H, cap)
     ws = codes.new_empty(nbytes) if nbytes else None      # partial states of the key splits
-    rc = _lib.lib().libra_bridge_attn_decode8(q.data_ptr(), q.stride(0), codes.data_ptr(), scales.data_ptr(), key_flag.data_ptr(),
-                                              key_flag.stride(0), query_flag.data_ptr(), kv_len.data_ptr(), _ptr(kv_start),
+    ldq, ldf = (q.stride(0), key_flag.stride(0)) if B > 1 else (H * 128, cap)        # (one row: its stride says nothing)
+    rc = _lib.lib().libra_bridge_attn_decode8(q.data_ptr(), ldq, codes.data_ptr(), scales.data_ptr(), key_flag.data_ptr(), ldf, query_flag.data_ptr(), kv_len.data_ptr(), _ptr(kv_start),
                                               out.data_ptr(), out.stride(0), B, H, cap, block, float(scale), _ptr(ws), nbytes,
                                               _stream())
     _lib.check(rc, "bridge_attn_decode8")

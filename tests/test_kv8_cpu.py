@@ -197,3 +197,30 @@ def test_rope_operands_are_refused(monkeypatch, name, what, bad):
 def test_rope_positions_are_refused(monkeypatch, name, bad):
     with pytest.raises(ValueError):
         _rope_call(monkeypatch, name, positions=bad)
+
+
+def test_one_row_of_any_stride_reaches_the_library(monkeypatch):
+    """A batch of one row whose stride is 1 (what a transpose leaves): the library is told the row's width instead."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from libra_amd import kernels as K
+    made = {}
+
+    class Library:
+        def __getattr__(self, fn):
+            return lambda *a: made.update({fn: a}) or 0
+    monkeypatch.setattr(K._lib, "lib", Library)
+    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    with FakeTensorMode():
+        e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+        u8, i32 = torch.uint8, torch.int32
+        row = lambda n, **kw: e(n, 1, **kw).t()  # noqa: E731
+        cache = e(4, 1, 2, 32, 128, dtype=u8), e(4, 1, 2, 2, dtype=u8)
+        assert row(256).stride() == (1, 1)
+        K.kv8_fill([row(256)] * 4, *cache, 1)
+        K.kv8_append([row(256)] * 4, *cache, e(1, dtype=torch.int64))
+        K.rope_bridge_pos_append8(row(768), row(16), *[e(256, 8)] * 4, e(1, dtype=u8), e(64, 128), e(64, 128), e(1, dtype=i32), 2, *cache, e(1, dtype=torch.int64))
+        K.bridge_attn_decode8(row(256), *cache, row(32, dtype=u8), e(1, dtype=u8), e(1, dtype=i32), 0.1)
+    assert made["libra_kv8_fill"][1:8:2] == made["libra_kv8_append"][1:8:2] == (256,) * 4
+    assert made["libra_rope_bridge_pos_append8"][1:4:2] == (768, 16)
+    assert (made["libra_bridge_attn_decode8"][1], made["libra_bridge_attn_decode8"][5]) == (256, 32)

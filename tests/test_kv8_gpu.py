@@ -311,3 +311,24 @@ def test_other_stream(K):
         got = K.bridge_attn_decode8(q, c2, s2, kf, qf, ln, 128 ** -0.5)
     side.synchronize()
     assert torch.equal(got, want)                       # quantising what was read back changes nothing the attention sees
+
+
+def test_one_row_of_any_stride(K):
+    """A single row's stride says nothing (torch leaves any number there, 1 after a transpose): a batch of one takes every row it is given."""
+    H, cap, D = 2, 32, 256
+    odd = lambda x: torch.as_strided(x, x.shape, (1, 1))  # noqa: E731
+    pair = [K.kv8_alloc(1, cap, H, "cuda", 16) for _ in range(2)]
+    kf, qf, ln = torch.zeros(1, cap, dtype=torch.uint8, device="cuda"), torch.ones(1, dtype=torch.uint8, device="cuda"), torch.full((1,), 3, dtype=torch.int32, device="cuda")
+    rows = [r.contiguous() for r in rows4(1, H, 21)]
+    new = [r.contiguous() for r in rows4(1, H, 22)]
+    g = torch.Generator().manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    w, cos, sin, qkv, tb = [rnd(D, 8) for _ in range(4)], rnd(64, 128), rnd(64, 128), rnd(1, 3 * D), rnd(1, 16)
+    outs = []
+    for c, f in zip(pair, (lambda x: x, odd)):
+        K.kv8_fill([f(r) for r in rows], *c, 1)
+        K.kv8_append([f(r) for r in new], *c, torch.tensor([1], device="cuda"))
+        x = qkv.clone()
+        K.rope_bridge_pos_append8(f(x), f(tb), *w, qf, cos, sin, ln, H, *c, torch.tensor([2], device="cuda"))
+        outs.append((x, K.bridge_attn_decode8(f(new[0]), *c, f(kf), qf, ln, 128 ** -0.5)))
+    assert all(torch.equal(a, b) for a, b in zip(pair[0] + outs[0], pair[1] + outs[1]))
