@@ -357,7 +357,7 @@ class KVCache:
         if dtype not in ("bf16", "fp8"):
             raise ValueError(f"KV cache dtype must be 'bf16' or 'fp8', got {dtype!r}")
         self.B, self.capacity, self.length = B, capacity, 0
-        self.dtype = dtype
+        self.dtype, self.block = dtype, block if dtype == "fp8" else None
         if dtype == "fp8":
             self.layers = [K.kv8_alloc(B, capacity, H // 128, device, block) for _ in range(layers)]           # (codes, scales)
             slots = K.round_up(capacity, block)

@@ -146,7 +146,7 @@ class LibraGenerationMixin:
             model_inputs = self.prepare_inputs_for_generation(input_ids, **model_kwargs)
             model_inputs.pop("past_hidden_states", None)
             model_inputs.pop("past_vision_flag", None)
-            cache_kw = {k: model_kwargs[k] for k in ("max_cache_len", "cache_dtype", "cache_block") if model_kwargs.get(k)}
+            cache_kw = {k: model_kwargs[k] for k in ("max_cache_len", "cache_dtype", "cache_block") if model_kwargs.get(k) is not None}
             outputs = self(**model_inputs, return_dict=True, **cache_kw)
             raw = outputs.logits[:, :, -1, :]
             nxt_scores = _run_all(logits_warper, input_ids, _run_all(logits_processor, input_ids, raw))

@@ -310,6 +310,8 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
                 raise ValueError("labels with use_cache / past_key_values: the cached path is inference only (:1142)")
             return self._forward_cached(input_ids, attention_mask, position_ids, past_key_values, contiguous_signal, vision_indices,
                                         max_cache_len, cache_dtype, cache_block)
+        if cache_dtype is not None or cache_block is not None:
+            raise ValueError("cache_dtype / cache_block without use_cache: this forward has no KV cache")
         if position_ids is not None:
             raise NotImplementedError("custom position_ids on the training path (positions are arange(S), :736-739)")
         B, S = lead.shape[1:3] if input_ids is not None else lead.shape[:2]
@@ -382,7 +384,7 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
         of this call) with the cached branch's rule that an EOI input token predicts nothing but a newline (:1141-1144).
         The KV cache holds `max_cache_len` tokens (default max_position_embeddings; generate() passes its max_length), as bf16 rows or
         with cache_dtype="fp8" in 8 bits (a scale for every `cache_block` tokens and head, default 16): half the memory and half the bytes
-        a step reads of it.  Both are chosen by the call that prefills; later steps go by the cache they are given."""
+        a step reads of it.  Both are chosen by the call that prefills; later steps go by the cache they are given (asking for another is an error)."""
         Q, B, S = input_ids.shape
         dims = self._dims
         # A decode step continues the generation its prefill started: the operand copies were checked and refreshed there, and
@@ -407,7 +409,9 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
                 if not torch.equal(position_ids.reshape(B, S).to(dev), want):
                     raise NotImplementedError("prefill positions other than attention_mask.cumsum(-1) - 1")
             cap = max(int(max_cache_len), S + 1) if max_cache_len else max(dims.max_pos, S + 1)
-            cache = DE.KVCache(dims.layers, B, cap, dims.hidden, dev, dtype=cache_dtype or "bf16",
+            if cache_block is not None and cache_dtype != "fp8":
+                raise ValueError(f"cache_block={cache_block} is the 8-bit cache's (cache_dtype='fp8'), got cache_dtype={cache_dtype!r}")
+            cache = DE.KVCache(dims.layers, B, cap, dims.hidden, dev, dtype="bf16" if cache_dtype is None else cache_dtype,
                                **({"block": cache_block} if cache_block is not None else {}))
             cache.pack_key = ptr_key
             cache.sd = sd
@@ -418,6 +422,9 @@ class LibraForCausalLM(LibraGenerationMixin, PreTrainedModel):
             if S != 1:
                 raise ValueError("only support generating token by token")             # cal_vision_logits_inference, :912
             cache = past
+            if cache_dtype is not None and cache_dtype != cache.dtype or cache_block is not None and cache_block != cache.block:
+                raise ValueError(f"cache_dtype={cache_dtype!r}, cache_block={cache_block}: the cache of this generation is {cache.dtype!r}"
+                                 + (f" with blocks of {cache.block}" if cache.block else "") + " (both are chosen by the call that prefills)")
             if cache.length >= cache.capacity:
                 raise ValueError(f"the KV cache is full ({cache.capacity} tokens): pass a larger max_cache_len / max_length")
             if cache.pack_key != ptr_key:                # parameter storage moved since the graphs were captured
