@@ -477,22 +477,15 @@ def layer_forward(sd, pk, i: int, d: DecDims, x, flag, lang_idx, vis_idx, lens, 
                               [sd[a + f"vision_{nm}_proj.weight_B"] for nm in ("q", "k", "v")],
                               [qkv[:, j * H:(j + 1) * H] for j in range(3)], c_rows=vis_idx)
     q8 = cache is not None and cache.dtype == "fp8"
-    fused_append = cache is not None and slot is not None and positions is not None
     bridge = (qkv, tb, pk["bk_l"], pk["bk_v"], pk["bv_l"], pk["bv_v"], flag, cos, sin)
-    if positions is None:
+    if slot is not None and q8:                             # decode step (always with positions): the new token's four cache rows
+        K.rope_bridge_pos_append8(*bridge, positions, d.heads, *cache.layers[i], slot)       # go out of the same launch
+    elif positions is not None:
+        kc, vc = K.rope_bridge_pos(*bridge, positions, d.heads, append=None if slot is None else (cache.layers[i], slot))
+    else:
         kc, vc = K.rope_bridge(*bridge, S, d.heads)
-    elif fused_append and q8:
-        K.rope_bridge_pos_append8(*bridge, positions, d.heads, *cache.layers[i], slot)
-    else:                                                   # (decode step: the new token's four cache rows go out of the same launch)
-        kc, vc = K.rope_bridge_pos(*bridge, positions, d.heads, append=(cache.layers[i], slot) if fused_append else None)
-    if cache is not None and not fused_append:              # the cache slots
-        new_rows = (qkv[:, H:2 * H], kc, qkv[:, 2 * H:], vc)
-        if slot is None:
-            cache.write_prompt(i, new_rows, S, kv_start)
-        elif q8:
-            K.kv8_append(new_rows, *cache.layers[i], slot)
-        else:
-            K.kv_cache_append(new_rows, cache.layers[i], slot)
+    if cache is not None and slot is None:                  # the prompt's cache slots
+        cache.write_prompt(i, (qkv[:, H:2 * H], kc, qkv[:, 2 * H:], vc), S, kv_start)
     if slot is None:
         o_lo = torch.empty((N, H), dtype=BF16, device=dev) if save else None   # rounding residual of o (the backward's D = dO.O)
         o, lse = K.bridge_attn_fwd(qkv[:, :H], qkv[:, H:2 * H], kc, qkv[:, 2 * H:], vc, flag, lens, B, S, d.heads,
