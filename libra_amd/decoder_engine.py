@@ -789,12 +789,12 @@ def score_heads(d: DecDims, labels, z_lang, z_vis, z_all, lang_idx, vis_idx, top
         for q in range(Q):
             if z_vis[q] is not None:
                 head(("vis", q), z_vis[q], slice(q, q + 1), vis_idx.long(), d.vocab)
-    scored = (tgt >= 0).float()
+    scored = tgt >= 0
 
     def shift(x, first):                                                            # row of token t - 1 -> position t
         x = x.view(Q, B, S, *x.shape[2:])
         return torch.cat([torch.full_like(x[:, :, :1], first), x[:, :, :-1]], 2)
-    return dict(logprobs=shift(lp, 0), entropy=shift(ent * scored, 0), top_ids=shift(ids, -1), top_logprobs=shift(tlp, float("-inf")),
+    return dict(logprobs=shift(lp, 0), entropy=shift(ent.masked_fill(~scored, 0), 0), top_ids=shift(ids, -1), top_logprobs=shift(tlp, float("-inf")),
                 parts=parts, scored=scored)
 
 
@@ -1023,7 +1023,7 @@ def backward(sd, packed, d: DecDims, out, want, gscale=1.0, g_scores=None):
         sc = {which: rest for which, *rest in sv["scores"]["parts"]}
         # back to the rows that predict: position t -> the row of token t - 1 (the last row predicts nothing)
         g_lp, g_en = (torch.cat([x[:, :, 1:], torch.zeros_like(x[:, :, :1])], 2).reshape(Q, N).contiguous() for x in g_scores)
-        g_en = g_en * sv["scores"]["scored"]
+        g_en = g_en.masked_fill(~sv["scores"]["scored"], 0)       # (selected, not multiplied: 0 * inf is no gradient of an unscored row)
     def head_pad(name):
         """Head weight with its vocab (the dgrad reduction length) zero-padded to the GEMM's 64 granule."""
         W = sd[name]

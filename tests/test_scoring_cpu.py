@@ -118,3 +118,15 @@ def test_a_backward_frees_the_call_and_is_the_only_one(monkeypatch):
     assert e.alive[0]() is None and p.grad.tolist() == [24.0] * 3          # (lp and ent are still held)
     with pytest.raises(RuntimeError, match="ran already"):
         both.backward()
+
+
+def test_rows_that_are_not_scored_answer_zero_whatever_they_hold(monkeypatch):
+    """A row whose logits are not finite and whose token is not scored: 0, not 0 * NaN."""
+    from libra_amd import kernels as K
+    monkeypatch.setattr(M.DE.K, "token_logprobs", lambda z, t, *, target_sub, top: K.TokenLogprobs(
+        torch.zeros(t.shape), torch.stack([z.amax(-1), z.sum(-1), z.mean(-1)]), (torch.zeros(len(z), top, dtype=torch.int64), torch.zeros(len(z), top))))
+    z = torch.tensor([[1.0, 3.0], [float("nan"), 0.0], [float("inf"), 0.0], [2.0, 4.0]])
+    labels = torch.tensor([[[0, 1, -100, -1]], [[0, -100, -100, 1]]])                  # the rows of tokens 0 .. 2 predict 1 .. 3
+    d = types.SimpleNamespace(vocab=2)
+    out = M.DE.score_heads(d, labels, z, [None, None], None, torch.arange(4, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), 1)
+    assert out["entropy"].tolist() == [[[0.0, 2.0, 0.0, 0.0]], [[0.0, 0.0, 0.0, float("inf")]]]

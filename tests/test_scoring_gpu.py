@@ -397,3 +397,23 @@ def test_scoring_leaves_nothing_behind():
         assert len(set(used[3:])) == 1, used            # (the first three bring the operands and the arena's buffers)
     finally:
         gc.enable()
+
+
+def test_gradients_at_positions_that_are_not_scored_are_dropped():
+    """sqrt(entropy) has an infinite derivative at the 0 of an unscored position: it belongs to a constant.  Bit for bit the gradient of the
+    same sum over the scored positions alone."""
+    m, _, t, c, _ = _model("default")
+    m.requires_grad_(True)
+    ids, lab, kw = t["in.input_ids"].cuda(), t["in.labels"].cuda(), _inputs(t)
+    on = lab >= 0
+    on[:, :, 0] = False
+    assert bool(on.any()) and not bool(on[:, :, 1:].all())
+    grads = []
+    for every in (False, True):
+        m.zero_grad()
+        out = m.token_logprobs(ids, lab, **kw)
+        (out.entropy if every else out.entropy[on]).sqrt().sum().backward()
+        grads.append({n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None})
+    assert grads[0].keys() == grads[1].keys() and len(grads[0]) > 50
+    for n, g in grads[0].items():
+        assert bool(torch.isfinite(g).all()) and torch.equal(g, grads[1][n]), n
