@@ -73,7 +73,12 @@ def _is_nccl(group) -> bool:
 
 
 def _staged(t: torch.Tensor, group) -> bool:
-    return t.is_cuda and not _is_nccl(group)
+    """Is `t` a device tensor that gloo would carry?  A group may hold a backend for each device type ("cpu:gloo,cuda:nccl", what a group
+    initialised without a backend gets, or "cuda:nccl" alone), so the question is which one `t`'s type has, not what the group is called."""
+    if not t.is_cuda:
+        return False
+    by_device = dict(pair.split(":", 1) for pair in str(dist.get_backend_config(group)).split(","))
+    return by_device.get(t.device.type) == "gloo"
 
 
 class _StagedWork:

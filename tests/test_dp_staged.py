@@ -82,3 +82,36 @@ def test_wait_copies_once():
     dst.add_(1)
     w.wait()
     assert Work.n == 1 and dst.tolist() == [2, 2, 2]
+
+
+@pytest.mark.parametrize("config,staged", [("cpu:gloo,cuda:gloo", True), ("cpu:gloo,cuda:nccl", False), ("cuda:nccl", False), ("cuda:nccl,cpu:gloo", False),
+                                           ("cpu:mpi,cuda:mpi", False)])
+def test_only_gloo_is_staged(config, staged, monkeypatch):
+    """What counts is the backend of the tensor's device type: a group initialised without a backend ("cpu:gloo,cuda:nccl") or for devices
+    only ("cuda:nccl") carries device tensors over RCCL, directly."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from libra_amd import dp
+    monkeypatch.setattr(dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(dist, "get_backend", lambda group=None: "undefined")
+    monkeypatch.setattr(dist, "get_backend_config", lambda group=None: config)
+    sent = []
+    work = object()
+    with FakeTensorMode():
+        t = torch.empty(8, device="cuda")
+        assert dp._staged(t, None) is staged and dp._staged(torch.empty(8), None) is False
+        if not staged:
+            assert dp._collective(lambda *ts, group, async_op: sent.extend(ts) or work, t) is work and sent == [t]
+
+
+def test_the_backend_of_a_real_group(monkeypatch):
+    """get_backend_config of the groups that can be made here names the backend of every device type."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from libra_amd import dp
+    for backend in ("gloo", "cpu:gloo,cuda:gloo", "cpu:gloo"):
+        dist.init_process_group(backend, init_method=f"tcp://127.0.0.1:{G._free_port()}", rank=0, world_size=1)
+        try:
+            with FakeTensorMode():
+                assert dp._staged(torch.empty(4, device="cuda"), None) is ("cuda" in backend or backend == "gloo")
+                assert dp._staged(torch.empty(4, device="cuda"), dist.group.WORLD) is ("cuda" in backend or backend == "gloo")
+        finally:
+            dist.destroy_process_group()
