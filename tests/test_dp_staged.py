@@ -115,3 +115,50 @@ def test_the_backend_of_a_real_group(monkeypatch):
                 assert dp._staged(torch.empty(4, device="cuda"), dist.group.WORLD) is ("cuda" in backend or backend == "gloo")
         finally:
             dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gather", [False, True])
+def test_device_copies_of_a_staged_collective(dtype, gather, monkeypatch):
+    """The copies themselves, one process and no group: what the collective is handed are host tensors with the values of the work queued on
+    the current stream until then; wait(), called with another stream current, leaves the result on the device for every stream."""
+    from libra_amd import dp
+    monkeypatch.setattr(dp, "_staged", lambda t, group: t.is_cuda)
+    n, dev = 100003, "cuda"
+    seen = []
+
+    class Work:
+        def __init__(self, done):
+            self.done = done
+
+        def wait(self):
+            self.done()
+
+    def collective(out, *inp, group, async_op, scale):
+        assert async_op and group is None and not out.is_cuda and not any(t.is_cuda for t in inp)
+        src = inp[0] if inp else out
+        seen.append(src.clone())
+
+        def done():
+            out.copy_(src.repeat(out.numel() // src.numel()) * scale)
+        return Work(done)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    a = torch.randint(-8, 9, (n,), generator=torch.Generator().manual_seed(0)).to(dtype)
+    big = torch.ones(2048, 2048, device=dev)
+    flat = torch.zeros(2 * n if gather else n, dtype=dtype, device=dev)
+    mine = flat[:n]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):                                             # (work in front of the values)
+            big = big @ big * 2.0 ** -11
+        mine.copy_(a.to(dev) * big[0, 0].to(dtype))
+        w = dp._collective(collective, flat, mine, scale=2) if gather else dp._collective(collective, flat, scale=2)
+    with torch.cuda.stream(other):
+        w.wait()
+        got = flat.clone()
+        flat.add_(1)
+        w.wait()                                                        # (a second wait copies nothing)
+    torch.cuda.synchronize()
+    assert torch.equal(seen[0], a) and torch.equal(got.cpu(), (2 * a).repeat(2 if gather else 1))
+    assert torch.equal(flat.cpu(), (2 * a).repeat(2 if gather else 1) + 1)
