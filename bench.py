@@ -362,9 +362,13 @@ def hbm_traffic(workload):
 def self_launch(n: int) -> int:
     """`python bench.py --gpus N` (N > 1) outside torchrun: re-run this command line as N ranks of one node under
     torch.distributed.run (one process per GPU, RCCL over xGMI; rendezvous on 127.0.0.1) and return its exit code.  Without this
-    the command would silently measure ONE GPU and report it as the N-GPU point of the scaling curve."""
+    the command would silently measure ONE GPU and report it as the N-GPU point of the scaling curve.
+    Every rank's stderr is also kept whole in a file of its own (under $LIBRA_RANK_LOGS, or a temporary folder that stays if a rank
+    fails), with Python's stacks where a rank ends in a signal: what an aborted rank said is not lost among the others' lines."""
+    import shutil
     import socket
     import subprocess
+    import tempfile
     backend = os.environ.get("LIBRA_DIST_BACKEND", "nccl")
     have = torch.cuda.device_count()
     if backend == "nccl" and have < n:
@@ -377,10 +381,18 @@ def self_launch(n: int) -> int:
     env = dict(os.environ)
     env.setdefault("HSA_ENABLE_IPC_MODE_LEGACY", "0")      # dmabuf IPC: RCCL's cross-process buffer sharing needs it on this driver
     env.setdefault("OMP_NUM_THREADS", "8")
+    env.setdefault("PYTHONFAULTHANDLER", "1")
+    kept = env.get("LIBRA_RANK_LOGS")
+    logs = kept or tempfile.mkdtemp(prefix="libra_bench_ranks_")
     cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={n}", "--master-addr", "127.0.0.1",
-           "--master-port", str(port), os.path.abspath(__file__)] + sys.argv[1:]
+           "--master-port", str(port), "--log-dir", logs, "--tee", "2", os.path.abspath(__file__)] + sys.argv[1:]      # (2: stderr only)
     print(f"[bench] launching {n} ranks: {' '.join(cmd[1:8])} ...", file=sys.stderr, flush=True)
-    return subprocess.run(cmd, env=env).returncode
+    rc = subprocess.run(cmd, env=env).returncode
+    if rc:
+        print(f"[bench] a rank failed (exit code {rc}); every rank's complete stderr is under {logs}", file=sys.stderr, flush=True)
+    elif not kept:
+        shutil.rmtree(logs, ignore_errors=True)
+    return rc
 
 
 def parse_showtopo(text: str):
