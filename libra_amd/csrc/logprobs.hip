@@ -457,7 +457,7 @@ __global__ __launch_bounds__(NT * ROWS) void logprobs_bwd_kernel(const LogprobBw
             const long long tg = p.targets[i * p.rows + row], v = tg - p.tsub;
             if (tg < 0) continue;
             g += p.g_lp[i * p.rows + row];
-            if (v >= p.V) continue;
+            if (v < 0 || v >= p.V) continue;                         // (in no column: only its -p, by g)
             const int c = (int)v / VEC, j = c / NT;
             if (c % NT == tid) hits |= 1ull << (j < 63 ? j : 63);
         }

@@ -203,6 +203,21 @@ def test_views_and_offsets(K, dtype):
             assert bool((buf[:, :3] == 9).all()) and bool((buf[:, 3 + V:] == 9).all())                # nothing beside it is touched
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradient_of_targets_below_the_head(K, dtype):
+    """Tokens whose column is negative, among them whole multiples of what a workgroup reads at a time: each counts with its -p, no column is
+    theirs, and the columns of the other given tokens are as ever."""
+    V, sub = 2100, 32000
+    z, _ = logits(6, V, 17, dtype)
+    t = torch.tensor([[sub - 1, sub - 256, sub - 512, sub - 1024, sub - 2048, 0], [sub, sub + 5, -1, sub - 8, sub + V - 1, sub + 300]], device="cuda")
+    g = torch.Generator().manual_seed(6)
+    g_lp, g_ent = torch.randn(2, 6, generator=g).cuda(), torch.randn(6, generator=g).cuda()
+    for w in (V, 514):
+        zw, tw = z[:, :w], t if w == V else t.where(t < sub + w, sub + w - 1)
+        out = check(K, zw, tw, sub, 3)
+        grad_check(zw, tw, sub, g_lp, g_ent, K.token_logprobs_bwd(zw, tw, out.stats, g_lp, g_ent, target_sub=sub))
+
+
 def test_many_targets_and_empty_calls(K):
     z, _ = logits(3, 50, 1, BF)
     t = torch.randint(0, 50, (64, 3), generator=torch.Generator().manual_seed(0)).cuda()
