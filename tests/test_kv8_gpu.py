@@ -332,3 +332,34 @@ def test_one_row_of_any_stride(K):
         K.rope_bridge_pos_append8(f(x), f(tb), *w, qf, cos, sin, ln, H, *c, torch.tensor([2], device="cuda"))
         outs.append((x, K.bridge_attn_decode8(f(new[0]), *c, f(kf), qf, ln, 128 ** -0.5)))
     assert all(torch.equal(a, b) for a, b in zip(pair[0] + outs[0], pair[1] + outs[1]))
+
+
+def attn_parts(K, B, H, cap, lens, seed):
+    """Attention of a batch and of each of its sequences alone: (batch, alone, the tolerance of either against the definition)."""
+    q, codes, scales, g = attn_case(K, B, H, cap, 16, seed)
+    kf = (torch.rand(B, cap, generator=g) < 0.4).to(torch.uint8).cuda()
+    qf = torch.tensor([i % 2 for i in range(B)], dtype=torch.uint8, device="cuda")
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    whole = attn_check(K, q, codes, scales, kf, qf, ln, None)
+    alone = torch.cat([attn_check(K, q[b:b + 1], codes[:, b:b + 1].contiguous(), scales[:, b:b + 1].contiguous(), kf[b:b + 1], qf[b:b + 1],
+                                  ln[b:b + 1], None) for b in range(B)])
+    return whole, alone
+
+
+def test_a_sequence_alone_and_in_a_batch_under_one_plan(K):
+    """Up to 1024 slots a (sequence, head) is one workgroup's whatever the batch: the same bits alone as in the batch."""
+    whole, alone = attn_parts(K, 4, 4, 512, [512, 333, 64, 500], 8)
+    assert torch.equal(whole, alone)
+    whole, alone = attn_parts(K, 3, 2, 1024, [1024, 1, 700], 9)
+    assert torch.equal(whole, alone)
+
+
+def test_a_sequence_alone_and_in_a_batch_under_two_plans(K):
+    """Larger caches split the keys of a small batch: alone a sequence's four heads take several workgroups each and the merge, in a batch of
+    64 one each.  Another order of the same fp32 sums: both are within the definition's tolerance (attn_check), so within twice it of each
+    other; the split is there to be crossed (other workspace sizes)."""
+    B, H, cap = 64, 4, 1552
+    L = K._lib.lib().libra_bridge_attn_decode8_workspace_bytes
+    assert L(B, H, cap) == 0 and L(1, H, cap) > 0
+    lens = [1552, 1537, 1536, 1025, 1024, 1023, 513, 512, 65, 64, 1, 0] + [37 * i % 1553 for i in range(52)]
+    attn_parts(K, B, H, cap, lens, 10)
