@@ -209,11 +209,18 @@ __global__ __launch_bounds__(256) void bridge_attn_decode8_merge_kernel(const De
 }
 
 // Key splits of a (sequence, head): 1 - no second kernel - where the pairs alone give every CU a workgroup; below that, as many as that
-// takes, of two iterations at least.  Workgroups of 8 waves, two a CU: of 4, 8 and 16 waves with 1 ... 32 splits the fastest or within
-// 4 % of it at every size tried; at 32 heads, us (waves x splits), HBM floor in brackets:
-//   8 x 1024 [12.9]: 15.4 (8x1) 15.3 (16x1) 19.1 (4x4)    16 x 2048 [51.6]: 50.0 (8x1) 53.3 (16x1) 50.6 (4x1)
-//   32 x 600 [30.2]: 31.8 (8x1) 40.9 (16x1) 31.7 (4x1)    64 x 2048 [206]: 181 (8x1) 189 (16x1) 189 (4x1)
-//   4 x 2048 [12.9]: 18.9 (8x2) 18.7 (16x1) 19.1 (4x4)    1 x 8191 [12.9]: 19.5 (8x8) 19.7 (16x8) 19.6 (4x16) 22.0 (4x32)
+// takes, at most one for two iterations of the CAPACITY (the lengths are device words: a captured step must not depend on them).
+// Workgroups of 8 waves, two a CU, measured against 4 and 16 waves with 1 ... 32 splits at 17 sizes of 32 heads.  us (waves x splits),
+// the rule's first, in brackets the bytes at the rate of a large copy (5.2 TB/s: what to expect, no bound - reads alone go faster):
+//   1 x 8191 [12.9]: 19.8 (8x8) 23.7 (8x4) 59.9 (8x1) 19.6 (4x16) 19.7 (16x8)    2 x 4000 [12.6]: 19.1 (8x4) 34.0 (8x1) 20.9 (8x8) 19.1 (16x4)
+//   4 x 2048 [12.9]: 18.8 (8x2) 20.7 (8x1) 19.5 (8x4) 18.7 (16x1)     8 x 1024 [12.9]: 15.8 (8x1) 20.9 (8x2) 15.3 (16x1) 19.1 (4x4)
+//   16 x 2048 [51.6]: 50.1 (8x1) 53.0 (8x2) 53.3 (16x1) 50.6 (4x1)    64 x 2048 [206]: 181 (8x1) 195 (8x2) 189 (16x1) 189 (4x1)
+//   32 x 600 [30.2]: 31.1 (8x1) 39.3 (8x2) 40.9 (16x1) 31.7 (4x1)
+// Within 4 % of the best at the sizes from 8 sequences on and at long contexts.  It is NOT the best where a small batch's contexts
+// are short of a capacity that splits (two splits share what one or two iterations hold, and the merge costs its launch), 2048 slots:
+//   1 x 300: 8.0 (8x2) 5.8 (8x1)    1 x 1024: 9.7 (8x2) 9.5 (8x1) 8.4 (4x4)    2 x 1024: 10.3 (8x2) 9.6 (8x1) 9.3 (4x4)
+//   4 x 1024: 13.8 (8x2) 13.7 (8x1) 12.2 (16x1)
+// The split decides the order of the fp32 sums: the same bits for the same (B H, capacity), and at any batch up to 1024 slots.
 static int d8_splits(int64_t B, int64_t H, int64_t capacity) {
     const int64_t want = (256 + B * H - 1) / (B * H), most = (capacity + 2 * D8_KEYS - 1) / (2 * D8_KEYS);
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), D8_MAX_SPLIT));

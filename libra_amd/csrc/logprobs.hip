@@ -7,7 +7,10 @@
 //   dz_v = sum_i g_i ([v = t_i] - p_v) - g_H p_v (log p_v + H),  and 1 - p_v at v = t_i as -expm1(log p_v).
 // HBM-bound where there are many large rows: V elements in (forward), V in and V out (backward) a row.  Measured, bf16: 8188 x 32000 in
 // 126 us (4.2 TB/s, VALU 64 % busy) and 189 us (5.5 TB/s); 16 x 32514 with 20 alternatives in 10 us (latency of one row's phases, 5
-// without alternatives); 9248 x 514 in 8 + 9 us (one generation of short waves).
+// without alternatives: threshold, listing and ranking wait for each other).  Short rows are bound by issue, not memory: 9248 x 514 in 8.1 +
+// 8.6 us for 9.5 and 19 MB.  A wave a row: 280 VALU instructions, of which the 9 columns a lane take some 95 (10.4 a column in long rows) -
+// the rest, two wave-wide reductions, log1p, statistics and targets, is paid by 64 lanes for one row - and 9248 waves are more than
+// the chip holds at a time (8192, 8 a SIMD), so a second, nearly empty generation follows.
 #include <algorithm>
 #include "hip_common.hpp"
 #include "../../include/libra_hip.h"
